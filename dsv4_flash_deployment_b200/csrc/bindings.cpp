@@ -882,6 +882,258 @@ void tp_argmax_merge(const Tensor& sync, const Tensor& peer_val, const Tensor& p
 }
 
 
+// ------------------------------------------------- norm_quant / gemm_i8 / logits
+// Numbers enter error messages as strings: with this toolchain's libstdc++ beside
+// torch's, streaming an integer from an extension crashes.
+std::string str(int64_t v) { return std::to_string(v); }
+std::string str(at::IntArrayRef s) {
+  std::string o = "[";
+  for (size_t i = 0; i < s.size(); ++i) o += (i ? ", " : "") + std::to_string(s[i]);
+  return o + "]";
+}
+std::string str(c10::Device d) {
+  return d.has_index() ? c10::DeviceTypeName(d.type(), true) + ":" + std::to_string((int)d.index())
+                       : c10::DeviceTypeName(d.type(), true);
+}
+
+int float_type(const Tensor& t, const char* what) {
+  switch (t.scalar_type()) {
+    case at::kBFloat16: return dsv4::F_BF16;
+    case at::kHalf: return dsv4::F_F16;
+    case at::kFloat: return dsv4::F_F32;
+    default: TORCH_CHECK(false, what, ": bf16, fp16 or fp32 expected, got ", c10::toString(t.scalar_type()));
+  }
+}
+
+void check_rows(const Tensor& t, const char* what, int64_t rows, int64_t cols, const Tensor& like) {
+  TORCH_CHECK(t.device() == like.device(), what, " must be on ", str(like.device()), ", got ", str(t.device()));
+  TORCH_CHECK(t.dim() == 2 && t.size(0) == rows && t.size(1) == cols && (t.stride(1) == 1 || cols <= 1), what,
+              ": [", str(rows), ", ", str(cols), "] with contiguous rows expected, got ", str(t.sizes()));
+  TORCH_CHECK(rows <= 1 || t.stride(0) >= cols, what, ": rows overlap");
+}
+
+void check_vec(const Tensor& t, const char* what, int64_t n, at::ScalarType ty, const Tensor& like) {
+  TORCH_CHECK(t.device() == like.device() && t.dim() == 1 && t.size(0) == n && t.scalar_type() == ty &&
+                  t.is_contiguous(),
+              what, ": contiguous ", c10::toString(ty), " [", str(n), "] on ", str(like.device()), " expected, got ",
+              c10::toString(t.scalar_type()), " ",
+              str(t.sizes()), " on ", str(t.device()));
+}
+
+uint32_t* err_word(const Tensor& err, const Tensor& like) {
+  TORCH_CHECK(err.device() == like.device() && err.scalar_type() == at::kInt && err.numel() >= 1, "error word");
+  return reinterpret_cast<uint32_t*>(err.data_ptr<int>());
+}
+
+// fmt: Q8Format.  w None: quantization only.  I8 / E4M3: q [T, D] 1-byte, scale fp32 [T];
+// MX8: q uint8 [>= T, D], scale uint8 chunks [>= ceil(T / 128), D / 128, 512].
+void norm_quant(const Tensor& x, const optional<Tensor>& res, const optional<Tensor>& res_out,
+                const optional<Tensor>& w, double eps, int64_t fmt, const Tensor& q, const Tensor& scale) {
+  CHECK_CUDA(x);
+  TORCH_CHECK(x.dim() == 2 && (x.stride(1) == 1 || x.size(1) <= 1), "x: [T, D] with contiguous rows");
+  const int64_t T = x.size(0), D = x.size(1);
+  TORCH_CHECK(D <= dsv4::kNormMaxD, "width ", str(D), ": at most ", str(dsv4::kNormMaxD));
+  TORCH_CHECK(T < (1ll << 31), "too many rows");
+  const int xt = float_type(x, "x");
+  dsv4::NormQuantParams p{};
+  p.T = (int)T;
+  p.D = (int)D;
+  p.x = x.data_ptr();
+  p.ldx = (size_t)x.stride(0);
+  if (res) {
+    check_rows(*res, "residual", T, D, x);
+    TORCH_CHECK(res->scalar_type() == x.scalar_type(), "residual: x's type expected");
+    p.res = res->data_ptr();
+    p.ldr = (size_t)res->stride(0);
+  }
+  if (res_out) {
+    TORCH_CHECK(res.has_value(), "residual_out without residual");
+    check_rows(*res_out, "residual_out", T, D, x);
+    TORCH_CHECK(res_out->scalar_type() == x.scalar_type(), "residual_out: x's type expected");
+    p.res_out = res_out->data_ptr();
+    p.ldro = (size_t)res_out->stride(0);
+    TORCH_CHECK((p.res_out != p.res || p.ldro == p.ldr || T <= 1) && (p.res_out != p.x || p.ldro == p.ldx || T <= 1),
+                "residual_out shares its start with an input of another row stride");
+  }
+  int wt = dsv4::F_F32;
+  if (w) {
+    wt = float_type(*w, "weight");
+    TORCH_CHECK(wt == xt || wt == dsv4::F_F32, "weight: x's type or fp32 expected");
+    check_vec(*w, "weight", D, w->scalar_type(), x);
+    TORCH_CHECK(eps >= 1e-30, "eps must be at least 1e-30");
+    p.w = w->data_ptr();
+    p.eps = (float)eps;
+  }
+  TORCH_CHECK(q.element_size() == 1 && q.device() == x.device(), "q: a 1-byte type on x's device");
+  if (fmt == dsv4::Q8_MX8) {
+    TORCH_CHECK(D % 128 == 0, "MXFP8 rows: width must be a multiple of 128");
+    TORCH_CHECK(q.dim() == 2 && q.size(0) >= T && q.size(1) == D && q.is_contiguous(), "q: contiguous [>= T, D]");
+    TORCH_CHECK(scale.device() == x.device() && scale.scalar_type() == at::kByte && scale.is_contiguous() &&
+                    scale.numel() >= (T + 127) / 128 * (D / 128) * 512,
+                "scale: uint8 chunks [ceil(T / 128), D / 128, 512]");
+    p.sf = scale.data_ptr<uint8_t>();
+  } else {
+    check_rows(q, "q", T, D, x);
+    check_vec(scale, "scale", T, at::kFloat, x);
+    p.scale = scale.data_ptr<float>();
+  }
+  p.q = reinterpret_cast<uint8_t*>(q.data_ptr());
+  p.ldq = (size_t)q.stride(0);
+  const c10::cuda::CUDAGuard guard(x.device());
+  CUDA_OK(dsv4::norm_quant(p, xt, w ? wt : (xt == dsv4::F_F32 ? dsv4::F_F32 : xt), (int)fmt, cur_stream()));
+}
+
+void dequant_rows(const Tensor& q, const Tensor& scale, int64_t fmt, const Tensor& out) {
+  CHECK_CUDA(q);
+  TORCH_CHECK(out.dim() == 2 && out.scalar_type() == at::kBFloat16, "out: bf16 [T, D]");
+  const int64_t T = out.size(0), D = out.size(1);
+  TORCH_CHECK(q.dim() == 2 && q.size(0) >= T && q.size(1) == D && (q.stride(1) == 1 || D <= 1) && q.element_size() == 1,
+              "q: 1-byte codes [>= T, D] with contiguous rows");
+  check_rows(out, "out", T, D, q);
+  const bool mx = fmt == dsv4::Q8_MX8;
+  if (mx) {
+    TORCH_CHECK(D % 128 == 0 && scale.device() == q.device() && scale.scalar_type() == at::kByte &&
+                    scale.is_contiguous() && scale.numel() >= (T + 127) / 128 * (D / 128) * 512,
+                "scale: uint8 chunks [ceil(T / 128), D / 128, 512]");
+  } else {
+    check_vec(scale, "scale", q.size(0), at::kFloat, q);
+  }
+  TORCH_CHECK(T < (1ll << 31) && D < (1ll << 31) && q.stride(0) < (1ll << 31) && out.stride(0) < (1ll << 31), "too large");
+  const c10::cuda::CUDAGuard guard(q.device());
+  CUDA_OK(dsv4::dequant_rows(reinterpret_cast<const uint8_t*>(q.data_ptr()), (int)q.stride(0),
+                             mx ? nullptr : scale.data_ptr<float>(), mx ? scale.data_ptr<uint8_t>() : nullptr, (int)T,
+                             (int)D, (int)fmt, ptr<bf16>(out), (int)out.stride(0), cur_stream()));
+}
+
+// Row stride of an int8 operand in bytes; TMA wants 16-byte row starts.
+size_t i8_stride(const Tensor& t, const char* what) {
+  const int64_t rows = t.size(0), k = t.size(1);
+  const int64_t ld = rows > 1 ? t.stride(0) : (k + 15) / 16 * 16;
+  TORCH_CHECK(ld % 16 == 0 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0, what,
+              ": rows must start on 16-byte boundaries (row stride a multiple of 16)");
+  return (size_t)ld;
+}
+
+void gemm_i8(const Tensor& x, const Tensor& xs, const Tensor& w, const Tensor& ws, const Tensor& out,
+             const Tensor& err) {
+  CHECK_CUDA(x);
+  TORCH_CHECK(x.dim() == 2 && w.dim() == 2, "x: [T, K], w: [N, K]");
+  const int64_t T = x.size(0), K = x.size(1), N = w.size(0);
+  TORCH_CHECK(x.scalar_type() == at::kChar && w.scalar_type() == at::kChar, "x and w: int8");
+  TORCH_CHECK(K >= 1 && K <= dsv4::kGemmI8MaxK, "K must be in 1..", str(dsv4::kGemmI8MaxK));
+  TORCH_CHECK(T < (1ll << 31) && N < (1ll << 31) - 128, "too many rows");
+  check_rows(x, "x", T, K, x);
+  check_rows(w, "w", N, K, x);
+  check_vec(xs, "x scale", T, at::kFloat, x);
+  check_vec(ws, "w scale", N, at::kFloat, x);
+  check_rows(out, "out", T, N, x);
+  const int ot = float_type(out, "out");
+  if (T == 0 || N == 0) return;
+  dsv4::GemmI8Params p{};
+  p.T = (int)T;
+  p.N = (int)N;
+  p.K = (int)K;
+  p.xs = xs.data_ptr<float>();
+  p.ws = ws.data_ptr<float>();
+  p.out = out.data_ptr();
+  p.ldo = (size_t)out.stride(0);
+  p.err = err_word(err, x);
+  const c10::cuda::CUDAGuard guard(x.device());
+  CUDA_OK(dsv4::gemm_i8(x.data_ptr<int8_t>(), i8_stride(x, "x"), w.data_ptr<int8_t>(), i8_stride(w, "w"), p, ot,
+                        num_sms(), cur_stream()));
+}
+
+// slots/repetition/frequency/presence/seen/counts together or none; bias_* together or
+// none; mask_row/mask together or none.
+void logits_rules(const Tensor& in, const Tensor& out, const optional<Tensor>& slots,
+                  const optional<Tensor>& repetition, const optional<Tensor>& frequency,
+                  const optional<Tensor>& presence, const optional<Tensor>& seen, const optional<Tensor>& counts,
+                  const optional<Tensor>& bias_off, const optional<Tensor>& bias_id, const optional<Tensor>& bias_val,
+                  const optional<Tensor>& mask_row, const optional<Tensor>& mask, const Tensor& err) {
+  CHECK_CUDA(in);
+  TORCH_CHECK(in.dim() == 2, "logits: [S, V]");
+  const int64_t S = in.size(0), V = in.size(1), words = (V + 31) / 32;
+  TORCH_CHECK(S <= 65535, "at most 65535 rows");
+  TORCH_CHECK(V < (1ll << 31) - 65536, "vocabulary too large");
+  const int ty = float_type(in, "logits");
+  check_rows(in, "logits", S, V, in);
+  check_rows(out, "out", S, V, in);
+  TORCH_CHECK(out.scalar_type() == in.scalar_type(), "out: the logits' type expected");
+  TORCH_CHECK(in.data_ptr() != out.data_ptr() || S <= 1 || in.stride(0) == out.stride(0),
+              "out shares the logits' memory with another row stride");
+  dsv4::LogitsRules p{};
+  p.S = (int)S;
+  p.V = (int)V;
+  p.in = in.data_ptr();
+  p.out = out.data_ptr();
+  p.ld_in = (size_t)in.stride(0);
+  p.ld_out = (size_t)out.stride(0);
+  p.words = (int)words;
+  if (slots) {
+    TORCH_CHECK(repetition && frequency && presence && seen && counts, "penalties need their parameters and a history");
+    check_vec(*slots, "slots", S, at::kInt, in);
+    check_vec(*repetition, "repetition", S, at::kFloat, in);
+    check_vec(*frequency, "frequency", S, at::kFloat, in);
+    check_vec(*presence, "presence", S, at::kFloat, in);
+    TORCH_CHECK(seen->scalar_type() == at::kInt && counts->scalar_type() == at::kInt && seen->is_contiguous() &&
+                    counts->is_contiguous(),
+                "history: contiguous int32 tables");
+    check_rows(*seen, "history bits", counts->size(0), words, in);
+    check_rows(*counts, "history counts", counts->size(0), V, in);
+    p.slots = slots->data_ptr<int>();
+    p.repetition = repetition->data_ptr<float>();
+    p.frequency = frequency->data_ptr<float>();
+    p.presence = presence->data_ptr<float>();
+    p.seen = seen->data_ptr<int>();
+    p.counts = counts->data_ptr<int>();
+    p.n_slots = (int)counts->size(0);
+  }
+  if (bias_off) {
+    TORCH_CHECK(bias_id && bias_val, "biases need token ids and values");
+    check_vec(*bias_off, "bias offsets", S + 1, at::kInt, in);
+    check_vec(*bias_id, "bias ids", bias_id->size(0), at::kInt, in);
+    check_vec(*bias_val, "bias values", bias_id->size(0), at::kFloat, in);
+    TORCH_CHECK(bias_id->size(0) < (1ll << 31), "too many biases");
+    p.bias_off = bias_off->data_ptr<int>();
+    p.bias_id = bias_id->data_ptr<int>();
+    p.bias_val = bias_val->data_ptr<float>();
+    p.n_bias = (int)bias_id->size(0);
+  }
+  if (mask) {
+    TORCH_CHECK(mask_row.has_value(), "masks need a mask row per logits row");
+    check_vec(*mask_row, "mask rows", S, at::kInt, in);
+    TORCH_CHECK(mask->device() == in.device() && mask->scalar_type() == at::kInt && mask->dim() == 2 &&
+                    mask->size(1) >= words && mask->stride(1) == 1 && mask->stride(0) < (1ll << 31),
+                "mask: int32 words [n, >= ", str(words), "] with contiguous rows");
+    p.mask_row = mask_row->data_ptr<int>();
+    p.mask = mask->data_ptr<int>();
+    p.n_masks = (int)mask->size(0);
+    p.ld_mask = (int)mask->stride(0);
+  }
+  p.err = err_word(err, in);
+  const c10::cuda::CUDAGuard guard(in.device());
+  CUDA_OK(dsv4::logits_rules(p, ty, cur_stream()));
+}
+
+void history_add(const Tensor& ids, const Tensor& slots, const Tensor& generated, const Tensor& seen,
+                 const Tensor& counts, const Tensor& err) {
+  CHECK_CUDA(counts);
+  TORCH_CHECK(counts.dim() == 2, "counts: [n_slots, V]");
+  const int64_t n = ids.numel(), V = counts.size(1), words = (V + 31) / 32;
+  TORCH_CHECK(n < (1ll << 31) && V < (1ll << 31), "too many tokens");
+  check_vec(ids, "ids", n, at::kInt, counts);
+  check_vec(slots, "slots", n, at::kInt, counts);
+  check_vec(generated, "generated", n, at::kInt, counts);
+  TORCH_CHECK(seen.scalar_type() == at::kInt && counts.scalar_type() == at::kInt && seen.is_contiguous() &&
+                  counts.is_contiguous(),
+              "history: contiguous int32 tables");
+  check_rows(seen, "history bits", counts.size(0), words, counts);
+  const c10::cuda::CUDAGuard guard(counts.device());
+  CUDA_OK(dsv4::history_add(ids.data_ptr<int>(), slots.data_ptr<int>(), generated.data_ptr<int>(), (int)n,
+                            seen.data_ptr<int>(), counts.data_ptr<int>(), (int)counts.size(0), (int)V, (int)words,
+                            err_word(err, counts), cur_stream()));
+}
+
 }  // namespace
 
 int64_t debug_bounds_attach(const Tensor& err) {
@@ -935,6 +1187,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("ep_dispatch", &ep_dispatch);
   m.def("ep_plan", &ep_plan);
   m.def("argmax_rows", &argmax_rows);
+  m.def("norm_quant", &norm_quant);
+  m.def("dequant_rows", &dequant_rows);
+  m.def("gemm_i8", &gemm_i8);
+  m.def("logits_rules", &logits_rules);
+  m.def("history_add", &history_add);
   m.def("tp_argmax_merge", &tp_argmax_merge);
   m.def("pdl_probe", &pdl_probe);
   m.def("ts_mark", &ts_mark);

@@ -45,6 +45,7 @@ enum KernelId : uint32_t {
   KID_COMM = 4,
   KID_MEGA = 5,
   KID_BOUNDS = 6,   // debug-bounds build: an index check failed (detail = site)
+  KID_LOGITS = 7,   // a slot (1), mask row (2) or history token (3) outside its table
 };
 
 DSV4_DEV void report_error(uint32_t* err, uint32_t code, uint32_t kid, uint32_t detail) {

@@ -87,5 +87,24 @@ cudaError_t gemm_launch(int kind, int epi, bool grouped, int bn, int bm, const A
 // elements; box = {128 bytes of K, box_rows}, 128B swizzle.
 enum TmaElem { TMA_U8 = 0, TMA_BF16 = 1, TMA_E2M1 = 2 };
 bool make_tma_2d(CUtensorMap* map, const void* base, int elem, uint64_t rows, uint64_t cols, uint32_t box_rows);
+// 2-D tensor map over [rows, cols] bytes, rows ld bytes apart (a multiple of 16; base
+// 16-byte aligned); what a 128 x box_rows tile has outside reads as zero.
+bool make_tma_rows_u8(CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols, uint64_t ld,
+                      uint32_t box_rows);
+
+// ---------------------------------------------------------- gemm_i8.cu
+struct GemmI8Params {
+  int T, N, K;          // tokens, output channels, inner dimension (1 .. 131071)
+  int t_tiles, n_tiles, k_tiles;   // set by gemm_i8
+  const float* xs;      // [T] scale per token
+  const float* ws;      // [N] scale per output channel
+  void* out;            // [T, N], rows ldo elements apart
+  size_t ldo;
+  uint32_t* err;
+};
+constexpr int kGemmI8MaxK = 131071;   // 2^14 * 131071 < 2^31: no sum of int8 products passes int32
+// x [T, K], w [N, K]: rows ldx / ldw bytes apart.  otype: FloatType (kernels.h)
+cudaError_t gemm_i8(const int8_t* x, size_t ldx, const int8_t* w, size_t ldw, GemmI8Params p, int otype, int sms,
+                    cudaStream_t st);
 
 }  // namespace dsv4

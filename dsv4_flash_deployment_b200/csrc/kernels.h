@@ -380,4 +380,59 @@ cudaError_t tp_argmax_merge(const PeerSync& s, const float* const* peer_val, con
 cudaError_t markov_step(const float* logits, int ld, int blk, int i, const float* mlog, int mld, int V, int n,
                         int* toks, int ts, const __nv_bfloat16* memb, int R, __nv_bfloat16* emb, cudaStream_t st);
 
+// -------------------------------------------------------- norm_quant.cu
+enum FloatType { F_BF16 = 0, F_F16 = 1, F_F32 = 2 };
+// 8-bit row formats: int8 or e4m3 with one fp32 scale per row, MXFP8 (e4m3 with a
+// ue8m0 scale per 32 columns, scale bytes in the GEMM's chunks)
+enum Q8Format { Q8_I8 = 0, Q8_E4M3 = 1, Q8_MX8 = 2 };
+constexpr int kNormMaxD = 32768;   // a row stays in one CTA's registers
+struct NormQuantParams {
+  int T, D;
+  const void* x;         // [T, D], rows ldx apart
+  size_t ldx;
+  const void* res;       // optional, x's type
+  size_t ldr;
+  void* res_out;         // optional (with res): x + res; may be x or res itself
+  size_t ldro;
+  const void* w;         // [D], or null: no norm, only the quantization of x (+ res)
+  float eps;
+  uint8_t* q;            // [T, D] codes, rows ldq apart
+  size_t ldq;
+  float* scale;          // [T] (I8, E4M3)
+  uint8_t* sf;           // scale chunks (MX8)
+};
+cudaError_t norm_quant(const NormQuantParams& p, int xtype, int wtype, int fmt, cudaStream_t st);
+cudaError_t dequant_rows(const uint8_t* q, int ldq, const float* scale, const uint8_t* sf, int T, int D, int fmt,
+                         __nv_bfloat16* y, int ldy, cudaStream_t st);
+
+// ------------------------------------------------------------ logits.cu
+struct LogitsRules {
+  int S, V;
+  const void* in;            // [S, V] logits, rows ld_in apart
+  void* out;                 // [S, V], rows ld_out apart; may be `in`
+  size_t ld_in, ld_out;
+  // penalties (null slots: none): row s reads the history of slots[s] (< 0: none)
+  const int* slots;
+  const float *repetition, *frequency, *presence;   // [S]
+  const int* seen;           // [n_slots, words] bit v: token v in the prompt or the output
+  const int* counts;         // [n_slots, V] occurrences in the output
+  int n_slots, words;
+  // biases (null bias_off: none): row s adds bias_val to the tokens bias_id, ascending,
+  // of entries bias_off[s] .. bias_off[s + 1]
+  const int *bias_off, *bias_id;
+  const float* bias_val;
+  int n_bias;
+  // masks (null mask: none): row s keeps the tokens whose bit is set in row mask_row[s]
+  // (< 0: all)
+  const int* mask_row;
+  const int* mask;           // [n_masks, mask_words], rows ld_mask words apart
+  int n_masks, ld_mask;
+  uint32_t* err;
+};
+cudaError_t logits_rules(const LogitsRules& p, int type, cudaStream_t st);
+// seen / counts of the tokens ids[i] in slots[i]; generated[i]: < 0 skips the token,
+// 0 marks it as the prompt's, > 0 counts it
+cudaError_t history_add(const int* ids, const int* slots, const int* generated, int n, int* seen, int* counts,
+                        int n_slots, int V, int words, uint32_t* err, cudaStream_t st);
+
 }  // namespace dsv4

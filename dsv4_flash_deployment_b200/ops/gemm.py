@@ -168,3 +168,61 @@ def prepare_w13(w1: torch.Tensor, s1: torch.Tensor, w3: torch.Tensor, s3: torch.
     else:
         w = w.view(torch.int8)
     return MxWeight.from_checkpoint(w, s, device)
+
+
+@dataclass
+class I8Weight:
+    """int8 weight ``[N, K]`` with one fp32 scale per output channel (row).  Rows start
+    on 16-byte boundaries (:meth:`from_quantized` pads them where they do not)."""
+
+    q: torch.Tensor          # int8 [N, K], row stride a multiple of 16
+    scale: torch.Tensor      # fp32 [N]
+
+    @staticmethod
+    def from_quantized(q: torch.Tensor, scale: torch.Tensor, device=None) -> "I8Weight":
+        device = device or q.device
+        if q.dtype != torch.int8 or q.dim() != 2 or scale.shape != (q.shape[0],):
+            raise ValueError(f"int8 [N, K] and scale [N] expected, got {q.dtype} {tuple(q.shape)}, {tuple(scale.shape)}")
+        n, k = q.shape
+        buf = torch.zeros(n, ceil_to(k, 16), dtype=torch.int8, device=device)[:, :k]
+        buf.copy_(q)
+        return I8Weight(buf, scale.to(device=device, dtype=torch.float32).contiguous())
+
+    @staticmethod
+    def from_float(w: torch.Tensor, device=None) -> "I8Weight":
+        """Symmetric per-channel quantization of ``w`` [N, K] (codes -127..127), a slice of
+        rows at a time."""
+        device = device or w.device
+        n, k = w.shape
+        q = torch.zeros(n, ceil_to(k, 16), dtype=torch.int8, device=device)[:, :k]
+        scale = torch.empty(n, device=device)
+        step = max(1, (1 << 26) // max(1, k))
+        for r in range(0, n, step):
+            q[r:r + step], scale[r:r + step] = N.row_quant(w[r:r + step].to(device).float(), "i8")
+        return I8Weight(q, scale)
+
+
+def gemm_i8(xq: torch.Tensor, xs: torch.Tensor, w: I8Weight, out: torch.Tensor | None = None,
+            out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """``out[t, n] = (sum_k xq[t, k] w.q[n, k]) * xs[t] * w.scale[n]``, the sum exact.
+
+    ``xq`` int8 [T, K] whose rows start on 16-byte boundaries (as
+    :func:`.norm.rms_norm_quant` writes them), ``xs`` fp32 [T]; K up to 131071; out
+    bf16, fp16 or fp32 ``[T, N]`` with contiguous rows."""
+    if out is None:
+        out = torch.empty(xq.shape[0], w.q.shape[0], dtype=out_dtype, device=xq.device)
+    if xq.is_cuda:
+        _ext.load().gemm_i8(xq, xs, w.q, w.scale, out, ErrorWord.get(xq.device))
+    else:
+        if xq.dtype != torch.int8 or xq.shape[1] != w.q.shape[1] or out.shape != (xq.shape[0], w.q.shape[0]):
+            raise RuntimeError("int8 x [T, K], w [N, K] and out [T, N] expected")
+        out.copy_(N.i8_linear(xq, xs, w.q, w.scale, out.dtype))
+    return out
+
+
+def linear_i8(x: torch.Tensor, w: I8Weight, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """Convenience (allocating) path: per-token int8 quantization, then the int8 product."""
+    from .norm import quantize_rows
+
+    xq, xs = quantize_rows(x, "i8")
+    return gemm_i8(xq, xs, w, out_dtype=out_dtype)

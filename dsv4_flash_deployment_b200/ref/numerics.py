@@ -174,6 +174,74 @@ def rms_norm(x: torch.Tensor, w: torch.Tensor, eps: float) -> torch.Tensor:
     return (y * w.to(torch.bfloat16).float()).to(x.dtype)
 
 
+I8_MAX = 127.0
+ROW_AMAX_FLOOR = 1e-30
+
+
+def row_quant(y: torch.Tensor, fmt: str) -> tuple[torch.Tensor, torch.Tensor]:
+    """fp32 rows -> 8 bits with one fp32 scale per row: ``"i8"`` (``scale = max|y| / 127``,
+    codes rounded to nearest) or ``"e4m3"`` (``max|y| / 448``).  A row with an
+    infinity or NaN gets a NaN scale and codes 0."""
+    top = I8_MAX if fmt == "i8" else FP8_MAX
+    bad = ~torch.isfinite(y).all(-1)
+    y = torch.where(bad[..., None], torch.zeros_like(y), y)
+    amax = y.abs().amax(-1).clamp_min(ROW_AMAX_FLOOR)
+    t = y * (top / amax)[..., None]
+    q = t.round().clamp(-top, top).to(torch.int8) if fmt == "i8" else t.clamp(-top, top).to(torch.float8_e4m3fn)
+    return q, torch.where(bad, torch.full_like(amax, float("nan")), amax / top)
+
+
+def add_rms_norm(x: torch.Tensor, w: torch.Tensor, eps: float,
+                 residual: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """(RMSNorm of x + residual in fp32, not rounded; the sum in ``x.dtype``)."""
+    s = x.float() if residual is None else x.float() + residual.float()
+    y = s * torch.rsqrt(s.square().mean(-1, keepdim=True) + eps) * w.float()
+    return y, s.to(x.dtype)
+
+
+def i8_linear(xq: torch.Tensor, xs: torch.Tensor, wq: torch.Tensor, ws: torch.Tensor,
+              out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """Exact int8 product sums, times the token's and the channel's scale in fp32."""
+    acc = xq.double() @ wq.double().t()          # sums below 2^53: exact
+    return (acc.float() * (xs[:, None] * ws[None, :])).to(out_dtype)
+
+
+def unpack_bits(words: torch.Tensor, n: int) -> torch.Tensor:
+    """int32 words [S, W] -> truth values [S, n]: bit j of word i is entry 32 i + j."""
+    b = (words[:, :, None] >> torch.arange(32, dtype=torch.int32, device=words.device)) & 1
+    return b.reshape(words.shape[0], -1)[:, :n] != 0
+
+
+def pack_bits(bits: torch.Tensor) -> torch.Tensor:
+    """Inverse of :func:`unpack_bits` (entries past the end are 0)."""
+    s, n = bits.shape
+    full = torch.zeros(s, (n + 31) // 32 * 32, dtype=torch.int64, device=bits.device)
+    full[:, :n] = bits
+    w = (full.view(s, -1, 32) << torch.arange(32, device=bits.device)).sum(-1)
+    return torch.where(w >= 1 << 31, w - (1 << 32), w).to(torch.int32)
+
+
+def logits_rules(logits: torch.Tensor, seen: torch.Tensor | None = None, counts: torch.Tensor | None = None,
+                 repetition: torch.Tensor | None = None, frequency: torch.Tensor | None = None,
+                 presence: torch.Tensor | None = None, bias: torch.Tensor | None = None,
+                 allowed: torch.Tensor | None = None) -> torch.Tensor:
+    """Penalties, then biases, then the mask, in fp32, rounded once to the logits'
+    type.  ``seen`` [S, V]: tokens of the prompt or the output; ``counts`` [S, V]:
+    occurrences in the output; ``bias`` [S, V] (-inf: banned); ``allowed`` [S, V]."""
+    z = logits.float()
+    neg = torch.full_like(z, float("-inf"))
+    if seen is not None:
+        rep = repetition[:, None]
+        z = torch.where(seen, torch.where(z > 0, z / rep, z * rep), z)
+        c = counts.float()
+        z = torch.where(counts > 0, z - (frequency[:, None] * c + presence[:, None]), z)
+    if bias is not None:
+        z = torch.where(bias == neg, neg, z + bias)
+    if allowed is not None:
+        z = torch.where(allowed, z, neg)
+    return z.to(logits.dtype)
+
+
 # ---------------------------------------------------------------------- rope
 def rope_inv_freqs(dim: int, original_seq_len: int, base: float, factor: float,
                    beta_fast: int, beta_slow: int) -> torch.Tensor:
