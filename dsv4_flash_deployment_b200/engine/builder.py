@@ -24,7 +24,7 @@ def build_model(cfg, device="cuda", max_tokens: int = 512, n_slots: int = 16, ma
                 ep=None, tp=None, experts_from: DSV4Model | None = None, kv_block: int = 0,
                 kv_pool_tokens: int = 0, engram_from: DSV4Model | None = None,
                 engram_shm: str | None = None, engram_token_map=None,
-                merge_shared: bool | None = None) -> DSV4Model:
+                merge_shared: bool | None = None, head_int8: bool = False) -> DSV4Model:
     """Builds the backbone.
 
     ``weights``: checkpoint dict (names of the reference checkpoint); None draws
@@ -47,7 +47,9 @@ def build_model(cfg, device="cuda", max_tokens: int = 512, n_slots: int = 16, ma
     hashes (``ref.engram.compressed_token_map``; None: ``id % C``).
     ``merge_shared``: the shared expert's tiles ride in the routed experts' grouped
     GEMMs where the layout allows it (None: ``DSV4_MERGE_SHARED``, default on;
-    False: two separate dense GEMMs).
+    False: two separate dense GEMMs).  ``head_int8``: the output head in 8-bit
+    integers with a scale per vocabulary entry (half the bytes read per step; the
+    log-probabilities are those of the quantized head).
     """
     dev = torch.device(device)
     if tp is not None and ep is not None:
@@ -90,7 +92,7 @@ def build_model(cfg, device="cuda", max_tokens: int = 512, n_slots: int = 16, ma
         head = tp.shard_head(head, cfg.vocab_size)
     model = DSV4Model(cfg, layers, embed, head, norm, max_tokens, n_slots, max_seq_len, dev, ep=ep,
                       head_vocab=cfg.vocab_size, tp=tp, kv_block=kv_block, kv_pool_tokens=kv_pool_tokens,
-                      merge_shared=merge_shared)
+                      merge_shared=merge_shared, head_int8=head_int8)
     if cfg.engram_layer_ids and engram_from is not None:
         eg = engram_from.engram
         if eg is None or eg.ring.shape[0] < n_slots + 1 or eg.rows.shape[0] < max_tokens:

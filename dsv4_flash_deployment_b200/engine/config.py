@@ -36,6 +36,7 @@ class EngineConfig:
                                             # fill this fraction of the GPU's memory (vLLM's flag)
     kv_preempt: bool = False                # paged caches: admit on the prompt's blocks, preempt (recompute)
                                             # the newest request when the pool runs short
+    head_int8: bool = False                 # output head in 8-bit integers (half its bytes per step)
     use_cuda_graphs: bool = True
     expert_storage_layers: int | None = None
     ep_transport: str = "nccl"              # "nccl" (baseline), "p2p" (NVLink peer stores) or "fused"

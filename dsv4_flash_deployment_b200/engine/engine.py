@@ -23,7 +23,7 @@ from typing import Iterable
 import torch
 
 from ..models.model import DSV4Model, SeqChunk, StepMeta
-from ..models.sampling import SamplingParams, logprob_entries
+from ..models.sampling import SamplingParams, TokenRules, logprob_entries
 from ..ops.gemm import ErrorWord
 from .scheduler import Request, Scheduler
 
@@ -59,7 +59,8 @@ class Engine:
               weights: dict | None = None, seed: int = 0, expert_storage_layers: int | None = None, ep=None,
               use_graphs: bool = True, chunk_size: int | None = None, extra_slots: int = 0, tp=None,
               experts_from=None, kv_block: int = 0, kv_pool_tokens: int = 0, engram_from=None,
-              engram_shm: str | None = None, engram_token_map=None, kv_preempt: bool = False) -> "Engine":
+              engram_shm: str | None = None, engram_token_map=None, kv_preempt: bool = False,
+              head_int8: bool = False) -> "Engine":
         """``extra_slots`` cache slots beyond ``max_seqs`` are kept out of the scheduler
         (the multi-rank control plane runs its 1-token join steps on one).  ``tp``:
         tensor-parallel group (every rank runs the same steps).  ``experts_from``: a
@@ -67,30 +68,48 @@ class Engine:
         ``kv_block`` / ``kv_pool_tokens``: paged compressed caches (admission then
         also waits for free blocks; ``kv_preempt``: optimistic admission with
         recompute preemption instead).  ``engram_token_map``: compressed token map of
-        the tokenizer for the Engram hashes (None: ``id % C``)."""
+        the tokenizer for the Engram hashes (None: ``id % C``).  ``head_int8``: the output
+        head in 8-bit integers (half its bytes per step)."""
         from .builder import build_model
         model = build_model(cfg, device, max_tokens=max_batched_tokens, n_slots=max_seqs + extra_slots,
                             max_seq_len=max_seq_len, weights=weights, seed=seed,
                             expert_storage_layers=expert_storage_layers, ep=ep, tp=tp, experts_from=experts_from,
                             kv_block=kv_block, kv_pool_tokens=kv_pool_tokens, engram_from=engram_from,
-                            engram_shm=engram_shm, engram_token_map=engram_token_map)
+                            engram_shm=engram_shm, engram_token_map=engram_token_map, head_int8=head_int8)
         return cls(model, max_seqs, max_batched_tokens, max_seq_len, chunk_size, use_graphs, preempt=kv_preempt)
 
     # ------------------------------------------------------------------- API
     def add_request(self, prompt: list[int], max_new_tokens: int, ignore_eos: bool = False,
                     stop_ids: Iterable[int] = (), temperature: float = 0.0, top_k: int = 0, top_p: float = 1.0,
-                    logprobs: int | None = None, seed: int | None = None) -> Request:
+                    logprobs: int | None = None, seed: int | None = None, **rules) -> Request:
         """``temperature`` 0 decodes greedily; > 0 samples softmax(logits / T),
         restricted to the ``top_k`` most likely tokens (0: all) and to the top-p
         nucleus (``top_p`` 1.0: all).  ``logprobs`` n >= 0: every generated token
         also carries its log-probability and the n most likely alternatives
         (``Request.logprobs``), from the raw logits.  ``seed``: the request's samples
         depend on (seed, position) only, so a seeded request repeats its output
-        whatever it is batched with."""
+        whatever it is batched with.  ``rules``: ``repetition_penalty``,
+        ``frequency_penalty``, ``presence_penalty``, ``logit_bias`` ({token id: value}),
+        ``allowed_token_ids`` or a ``grammar`` object (models/sampling.py
+        :class:`TokenRules`), greedy or not."""
         sp = self.sampling_params(temperature, top_k, top_p, logprobs, seed)
+        tr = self.token_rules(**rules)
         return self.sched.add(prompt, max_new_tokens, ignore_eos=ignore_eos, eos_id=self.eos_id,
                               stop_ids=tuple(stop_ids), temperature=sp.temperature, top_k=sp.top_k, top_p=sp.top_p,
-                              want_logprobs=sp.logprobs, seed=sp.seed)
+                              want_logprobs=sp.logprobs, seed=sp.seed, rules=tr)
+
+    def token_rules(self, **rules) -> TokenRules | None:
+        """Checked rules on a request's logits (ValueError when this engine cannot apply
+        them: they need the whole vocabulary's logits on one GPU)."""
+        unknown = set(rules) - {"repetition_penalty", "frequency_penalty", "presence_penalty", "logit_bias",
+                                "allowed_token_ids", "grammar"}
+        if unknown:
+            raise TypeError(f"unknown decoding options: {sorted(unknown)}")
+        tr = TokenRules.make(self.cfg.vocab_size, **rules)
+        if tr is not None and getattr(self.model, "tp", None) is not None:
+            raise ValueError("penalties / logit_bias / grammars are not supported with the tensor-parallel "
+                             "(vocab-parallel) head")
+        return tr
 
     def sampling_params(self, temperature: float = 0.0, top_k: int = 0, top_p: float = 1.0,
                         logprobs: int | None = None, seed: int | None = None) -> SamplingParams:
@@ -109,7 +128,8 @@ class Engine:
             return []
         meta = StepMeta(self.cfg, [SeqChunk(c.req.slot, c.start_pos, c.tokens, c.sample,
                                             temperature=c.req.temperature, top_k=c.req.top_k, top_p=c.req.top_p,
-                                            logprobs=c.req.want_logprobs, seed=c.req.seed) for c in chunks])
+                                            logprobs=c.req.want_logprobs, seed=c.req.seed, **self._rules_of(c))
+                                   for c in chunks])
         ids = self.run_meta(meta)
         if meta.want_lp:
             it = iter(self.last_logprobs)
@@ -119,6 +139,19 @@ class Engine:
                     if e is not None:
                         c.req.logprobs.append(e)
         return self.sched.commit(chunks, ids)
+
+    def _rules_of(self, c) -> dict:
+        r = c.req.rules
+        if r is None:
+            return {}
+        mask = None
+        if c.sample:
+            try:
+                mask = r.words(c.req.output, self.cfg.vocab_size, self.eos_id)
+            except Exception as e:  # noqa: BLE001  (a request's own grammar object: only that request ends)
+                c.req.error = f"grammar: {type(e).__name__}: {e}"
+                self.sched.cancel(c.req)
+        return {"rules": r, "n_prompt": len(c.req.prompt), "mask": mask}
 
     last_logprobs: list = []   # per sampled row of the last step that asked for log-probabilities
 
@@ -200,7 +233,7 @@ class Engine:
     def generate(self, prompts: list[list[int]], max_new_tokens: int, ignore_eos: bool = False,
                  **sampling) -> list[list[int]]:
         """Runs the prompts to completion; ``sampling``: :meth:`add_request`'s decoding
-        options (temperature, top_k, top_p, seed, logprobs)."""
+        options (temperature, top_k, top_p, seed, logprobs, penalties, biases, grammar)."""
         reqs = [self.add_request(p, max_new_tokens, ignore_eos, **sampling) for p in prompts]
         while not all(r.finished for r in reqs):
             self.step()

@@ -43,6 +43,8 @@ class Request:
     top_p: float = 1.0                # 1.0 = off
     want_logprobs: int | None = None  # alternatives per generated token (None: no log-probabilities)
     seed: int | None = None           # samples depend on (seed, position) only
+    rules: object = None              # models.sampling.TokenRules: penalties, biases, grammar
+    error: str | None = None          # why the engine cancelled it (a grammar that failed)
     slot: int = -1
     n_prefilled: int = 0
     output: list[int] = field(default_factory=list)

@@ -31,12 +31,15 @@ import numpy as np
 import torch
 
 from ..ops import _ext
-from ..ops.gemm import (EPI_BF16, EPI_F32, EPI_SWIGLU, ErrorWord, MxWeight, gemm_bf16, gemm_mx,
+from ..ops.gemm import (EPI_BF16, EPI_F32, EPI_SWIGLU, ErrorWord, I8Weight, MxWeight, gemm_bf16, gemm_i8, gemm_mx,
                         pick_bn)
 from ..ops.layout import ceil_to
+from ..ops.logits import RowRules, TokenHistory, apply_logits_rules
+from ..ops.norm import empty_rows, rms_norm_quant
 from ..ref import numerics as N
 from .kv_format import ik4_bytes, kv4_bytes, kv8_bytes
-from .sampling import LOGPROB_TOP_N, chosen_logprob, gumbel_, logprob_top, seed_key, top_k_top_p_mask_
+from .sampling import (LOGPROB_TOP_N, MAX_BIAS, TokenRules, chosen_logprob, gumbel_, logprob_top, seed_key,
+                       top_k_top_p_mask_)
 from .weights import LayerW
 
 ROUTER_SMALL_T = 4   # steps of at most this many tokens route with csrc/moe.cu router_small
@@ -57,6 +60,9 @@ class SeqChunk:
     top_p: float = 1.0         # < 1: sample within the top-p nucleus only (temperature > 0)
     logprobs: int | None = None  # n >= 0: also return the sampled token's log-probability and n alternatives
     seed: int | None = None    # samples depend on (seed, position) only (temperature > 0)
+    rules: TokenRules | None = None   # penalties, biases, grammar of the sampled token
+    n_prompt: int = 0          # with rules: tokens at positions from here on are output
+    mask: np.ndarray | None = None    # grammar mask words of the sampled token (TokenRules.words)
 
 
 class StepMeta:
@@ -129,6 +135,7 @@ class StepMeta:
             self.lp_want = [None] * S
         self.seeded = bool((self.has_seed & (self.temps > 0)).any())
         self.want_lp = any(w is not None for w in self.lp_want)
+        self._rule_rows(n, lens, per_chunk, T)
         self.max_pos = int(self.pos.max()) if T else 0
         # compressor groups closed in this step, per ratio (token order)
         self.groups = {}
@@ -138,6 +145,52 @@ class StepMeta:
                               self.step_row0[mask])
         self.clen = {r: ((self.pos + 1) // r).astype(np.int32) for r in self.groups}
         self._lens = lens
+
+    def _rule_rows(self, n: int, lens, per_chunk, T: int) -> None:
+        """Rules on logits: ``hist`` per token (-1: not recorded, 0: prompt, 1: output),
+        and per sampled row the history slot, the penalties, the mask row and the
+        biases (``bias_off`` into ``bias_ids`` / ``bias_vals``)."""
+        chunks = self.chunks
+        self.ruled = any(c.rules is not None for c in chunks)
+        self.resets: list[int] = []     # slots whose history starts over in this step
+        if not self.ruled:
+            return
+        S = len(self.sample_rows)
+        self.hist = np.full(T, -1, np.int32)
+        self.r_slot = np.full(S, -1, np.int32)
+        self.r_rep = np.ones(S, np.float32)
+        self.r_freq = np.zeros(S, np.float32)
+        self.r_pres = np.zeros(S, np.float32)
+        self.mask_rows = np.full(S, -1, np.int32)
+        self.masks: list[np.ndarray] = []
+        off = np.zeros(S + 1, np.int64)
+        ids, vals = [], []
+        t0 = s0 = 0
+        for c, ln, k in zip(chunks, lens.tolist(), per_chunk.tolist()):
+            r = c.rules
+            if r is not None:
+                if c.sample_all:
+                    raise ValueError("rules on logits apply to one sampled token per sequence and step")
+                if r.penalizes:
+                    self.hist[t0:t0 + ln] = np.arange(c.start_pos, c.start_pos + ln) >= c.n_prompt
+                    if c.start_pos == 0:
+                        self.resets.append(c.slot)
+                if k:
+                    if r.penalizes:
+                        self.r_slot[s0] = c.slot
+                        self.r_rep[s0], self.r_freq[s0], self.r_pres[s0] = r.repetition, r.frequency, r.presence
+                    if c.mask is not None:
+                        self.mask_rows[s0] = len(self.masks)
+                        self.masks.append(c.mask)
+                    off[s0 + 1] = len(r.bias)
+                    for t, b in r.bias:
+                        ids.append(t)
+                        vals.append(b)
+            t0 += ln
+            s0 += int(k)
+        self.bias_off = np.cumsum(off).astype(np.int32)
+        self.bias_ids = np.array(ids, np.int32)
+        self.bias_vals = np.array(vals, np.float32)
 
     def index_bypass(self, r: int) -> bool:
         """True when every token's compressed length <= index_topk: top-k selects all."""
@@ -162,7 +215,7 @@ class StepMeta:
         nothing else, so steps of different batch compositions share a graph."""
         return (self.T, len(self.sample_rows), self.chunk_bound,
                 tuple(self.index_bypass(r) for r in self.groups), self.sampling, self.filtering, self.want_lp,
-                self.seeded)
+                self.seeded, self.ruled)
 
     def padded(self, max_tokens: int, max_sample: int, pad_slot: int) -> "StepMeta":
         """This step padded to bucketed shapes (:func:`token_bucket`): a padding chunk
@@ -189,6 +242,13 @@ class StepMeta:
             m.lp_want = m.lp_want + [None] * extra
             m.has_seed = np.concatenate([m.has_seed, np.zeros(extra, bool)])
             m.seedkey = np.concatenate([m.seedkey, np.zeros(extra, np.int64)])
+            if m.ruled:     # no rule acts on the extra rows
+                m.r_slot = np.concatenate([m.r_slot, np.full(extra, -1, np.int32)])
+                m.r_rep = np.concatenate([m.r_rep, np.ones(extra, np.float32)])
+                m.r_freq = np.concatenate([m.r_freq, np.zeros(extra, np.float32)])
+                m.r_pres = np.concatenate([m.r_pres, np.zeros(extra, np.float32)])
+                m.mask_rows = np.concatenate([m.mask_rows, np.full(extra, -1, np.int32)])
+                m.bias_off = np.concatenate([m.bias_off, np.full(extra, m.bias_off[-1], np.int32)])
         m.n_out = S
         return m
 
@@ -209,8 +269,11 @@ class DSV4Model:
     def __init__(self, cfg, layers: list[LayerW], embed: torch.Tensor, head: torch.Tensor, norm_w: torch.Tensor,
                  max_tokens: int, n_slots: int, max_seq_len: int, device, ep=None, max_sample: int | None = None,
                  head_vocab: int | None = None, tp=None, kv_block: int = 0, kv_pool_tokens: int = 0,
-                 merge_shared: bool | None = None):
+                 merge_shared: bool | None = None, head_int8: bool = False):
         self.cfg = cfg
+        # int8 output head: per-channel weights, per-token activations (half the bytes of the
+        # bf16 head, which every step reads whole)
+        self.head_q = I8Weight.from_float(head) if head_int8 else None
         self._want_merge = merge_shared
         self.layers = layers
         self.dev = torch.device(device)
@@ -354,6 +417,8 @@ class DSV4Model:
         self.router_counter = z(1, dt=i32)   # router_small's last-CTA counter (left at zero)
         # head
         self.u_sample = e(self.max_sample, D)
+        if self.head_q is not None:
+            self.u_sample_q, self.u_sample_s = empty_rows(self.max_sample, D, "i8", dev)
         self.logits = e(self.max_sample, self.head.shape[0], dt=f32)
         self.next_ids = e(self.max_sample, dt=i32)
         self.m_temp = z(self.max_sample, dt=f32)
@@ -466,12 +531,49 @@ class DSV4Model:
         if m.seeded:
             put(self.m_seedkey, m.seedkey)
             put(self.m_hasseed, m.has_seed)
+        if m.ruled:
+            self._upload_rules(m, put)
         for r, g in m.groups.items():
             for dst, arr in zip(self.m_groups[r], g):
                 if len(arr):
                     put(dst, arr)
             put(self.m_clen[r], m.clen[r])
             put(self.m_ngroups[r], np.asarray([len(g[0])], np.int32))
+
+    history: TokenHistory | None = None     # tokens of every slot, for penalties
+
+    def _upload_rules(self, m: StepMeta, put) -> None:
+        """Rules of the sampled rows; the buffers are made by the first step that has any."""
+        if self.history is None:
+            dev, S, V = self.dev, self.max_sample, self.vocab
+            i32, f32 = torch.int32, torch.float32
+            self.history = TokenHistory.empty(self.n_slots + 1, V, dev)
+            self.m_hist = torch.empty(self.max_tokens, dtype=i32, device=dev)
+            self.r_slot = torch.empty(S, dtype=i32, device=dev)
+            self.r_pen = tuple(torch.empty(S, dtype=f32, device=dev) for _ in range(3))
+            self.r_mask_rows = torch.empty(S, dtype=i32, device=dev)
+            self.r_masks = torch.empty(S * ((V + 31) // 32), dtype=i32, device=dev)
+            self.r_bias_off = torch.empty(S + 1, dtype=i32, device=dev)
+            self.r_bias_ids = torch.zeros(S * MAX_BIAS, dtype=i32, device=dev)
+            self.r_bias_vals = torch.zeros(S * MAX_BIAS, dtype=f32, device=dev)
+        for slot in m.resets:
+            self.history.reset(slot)
+        put(self.m_hist, m.hist)
+        put(self.r_slot, m.r_slot)
+        for dst, arr in zip(self.r_pen, (m.r_rep, m.r_freq, m.r_pres)):
+            put(dst, arr)
+        put(self.r_mask_rows, m.mask_rows)
+        put(self.r_bias_off, m.bias_off)
+        if len(m.bias_ids):
+            put(self.r_bias_ids, m.bias_ids)
+            put(self.r_bias_vals, m.bias_vals)
+        if m.masks:
+            put(self.r_masks, np.concatenate(m.masks))
+
+    def _row_rules(self, S: int) -> RowRules:
+        return (RowRules().penalties(self.r_slot[:S], *(t[:S] for t in self.r_pen))
+                .biases(self.r_bias_off[:S + 1], self.r_bias_ids, self.r_bias_vals)
+                .masks(self.r_mask_rows[:S], self.r_masks.view(self.max_sample, -1)))
 
     last_upload_bytes = 0
     op_timer: dict | None = None
@@ -596,22 +698,34 @@ class DSV4Model:
             moe_state = self._moe(L, T)
         # final collapse + norm on all tokens, then head on the sampled rows
         yp, ps, kk, td = moe_state
+        # (the int8 head takes the collapse, norms the sampled rows only and quantizes them)
         self._hc(T, Y=self.shared_y, yperm=yp, pos=ps, topk=kk, prev=self.mixF, mixes=None, cw=self.mixF,
-                 norm=self.norm_w, u=self.u, tp=td)
+                 norm=self.norm_w, u=self.u if self.head_q is None else None, tp=td)
         S = len(m.sample_rows)
+        if m.ruled:     # this step's tokens join their slots' histories before any row reads them
+            self.history.add(self.m_ids[:T], self.m_slot[:T], self.m_hist[:T])
         if S == 0:
             return self.next_ids[:0]
         with self._t("head"):
-            torch.index_select(self.u[:T], 0, self.m_sample[:S], out=self.u_sample[:S])
-            self._gemm_bf16(self.u_sample[:S], self.head, self.logits[:S], S, f32_out=True)
-            if (m.filtering or m.want_lp) and self.tp is not None:
-                raise NotImplementedError("top-k / top-p / log-probabilities with the vocab-parallel head")
+            if self.head_q is None:
+                torch.index_select(self.u[:T], 0, self.m_sample[:S], out=self.u_sample[:S])
+                self._gemm_bf16(self.u_sample[:S], self.head, self.logits[:S], S, f32_out=True)
+            else:
+                torch.index_select(self.hc_c[:T], 0, self.m_sample[:S], out=self.u_sample[:S])
+                q, sc = rms_norm_quant(self.u_sample[:S], self.norm_w, cfg.rms_norm_eps, "i8",
+                                       q_out=self.u_sample_q[:S], scale_out=self.u_sample_s[:S])
+                gemm_i8(q, sc, self.head_q, self.logits[:S])
+            if (m.filtering or m.want_lp or m.ruled) and self.tp is not None:
+                raise NotImplementedError("top-k / top-p / log-probabilities / rules on logits with the "
+                                          "vocab-parallel head")
             if m.want_lp:
                 raw = self._raw_logits(S)
                 n_top = min(LOGPROB_TOP_N, self.vocab)
                 lse, vals, ids = logprob_top(raw, n_top)
                 self.lp_vals[:S, :n_top].copy_(vals)
                 self.lp_ids[:S, :n_top].copy_(ids)
+            if m.ruled:
+                apply_logits_rules(self.logits[:S, :self.vocab], self._row_rules(S), self.history)
             if m.filtering:
                 top_k_top_p_mask_(self.logits[:S, :self.vocab], self.m_temp[:S], self.m_topk[:S], self.m_topp[:S])
             if m.sampling:

@@ -15,6 +15,7 @@ from __future__ import annotations
 
 import torch
 
+from ..ops.logits import RowRules, TokenHistory, apply_logits_rules
 from ..ref.model import RefModel, RefState
 from .model import StepMeta
 from .sampling import LOGPROB_TOP_N, chosen_logprob, logprob_top, seed_key, seeded_gumbel, top_k_top_p_mask_
@@ -29,6 +30,19 @@ class OracleStepModel:
         self.states: list[RefState | None] = [None] * n_slots
         self.last_upload_bytes = 0
         self._gen = torch.Generator().manual_seed(0)
+        self.history: TokenHistory | None = None
+
+    def _rules(self, c, lg: torch.Tensor) -> None:
+        """The chunk's rules on its sampled row, in place."""
+        i32 = lambda v: torch.tensor(v, dtype=torch.int32)
+        r, rows = c.rules, RowRules()
+        if r.penalizes:
+            rows.penalties(i32([c.slot]), *(torch.tensor([x]) for x in (r.repetition, r.frequency, r.presence)))
+        if r.bias:
+            rows.biases(i32([0, len(r.bias)]), i32([t for t, _ in r.bias]), torch.tensor([b for _, b in r.bias]))
+        if c.mask is not None:
+            rows.masks(i32([0]), torch.from_numpy(c.mask.copy())[None])
+        apply_logits_rules(lg, rows, self.history)
 
     def upload(self, meta: StepMeta, pinned: dict | None = None) -> None:
         self.last_upload_bytes = 0
@@ -45,12 +59,22 @@ class OracleStepModel:
                 self.states[c.slot] = st
             if st.pos != c.start_pos:
                 raise RuntimeError(f"slot {c.slot}: state at {st.pos}, chunk starts at {c.start_pos}")
+            if c.rules is not None and c.rules.penalizes:
+                if self.history is None:
+                    self.history = TokenHistory.empty(len(self.states), self.cfg.vocab_size, "cpu")
+                if c.start_pos == 0:
+                    self.history.reset(c.slot)
+                i32 = lambda v: torch.tensor(v, dtype=torch.int32)
+                self.history.add(i32(c.tokens), i32([c.slot] * len(c.tokens)),
+                                 i32([int(c.start_pos + j >= c.n_prompt) for j in range(len(c.tokens))]))
             logits = None
             for tok in c.tokens:
                 logits, _ = self.ref.step(torch.tensor([tok]), st)
             if c.sample:
                 lg = logits[0].float()[None, : self.cfg.vocab_size].clone()
                 raw = lg.clone()
+                if c.rules is not None:
+                    self._rules(c, lg)
                 temp = torch.tensor([c.temperature])
                 if c.temperature > 0 and (c.top_k > 0 or c.top_p < 1.0):
                     top_k_top_p_mask_(lg, temp, torch.tensor([c.top_k], dtype=torch.int32),

@@ -18,11 +18,118 @@ reaches ``p`` (at least one token).
 
 from __future__ import annotations
 
+import math
 from dataclasses import dataclass
 
+import numpy as np
 import torch
 
 LOGPROB_TOP_N = 20   # most alternatives a request may ask for (the OpenAI API's top_logprobs limit)
+MAX_BIAS = 300       # most biased tokens of a request (the limit vLLM's and OpenAI's servers document)
+
+
+class AllowedTokens:
+    """The simplest grammar: only the tokens of a list, at every position.
+
+    A grammar is any object with ``mask(output)``: the int32 words (bit j of word i =
+    token 32 i + j, at least ceil(V / 32) of them) of the tokens that may follow the
+    tokens generated so far, or None where any may."""
+
+    def __init__(self, token_ids, vocab: int):
+        ids = sorted({int(t) for t in token_ids})
+        if not ids or ids[0] < 0 or ids[-1] >= vocab:
+            raise ValueError("allowed_token_ids: a list of token ids of the vocabulary")
+        self._words = token_words(ids, vocab)
+
+    def mask(self, output):
+        return self._words
+
+
+def token_words(ids, vocab: int) -> np.ndarray:
+    """Mask words with the bits of ``ids`` set."""
+    bits = np.zeros((vocab + 31) // 32 * 32, np.uint8)
+    bits[np.asarray(ids, np.int64)] = 1
+    return np.packbits(bits, bitorder="little").view("<u4").astype(np.uint32).view(np.int32)
+
+
+@dataclass(frozen=True)
+class TokenRules:
+    """What a request does to its logits before they are sampled (greedy or not), in
+    this order (:mod:`..ops.logits`): ``repetition`` divides the positive and multiplies
+    the other logits of tokens in the prompt or the output (1: off); ``frequency`` times
+    its count and ``presence`` are taken off a token of the output; ``bias`` (pairs of
+    token id and value, -inf bans) is added; ``grammar`` (:class:`AllowedTokens`) bans
+    what it does not allow.  Log-probabilities stay those of the raw logits."""
+
+    repetition: float = 1.0
+    frequency: float = 0.0
+    presence: float = 0.0
+    bias: tuple[tuple[int, float], ...] = ()
+    grammar: object = None
+
+    @property
+    def penalizes(self) -> bool:
+        return self.repetition != 1.0 or self.frequency != 0.0 or self.presence != 0.0
+
+    @staticmethod
+    def make(vocab: int, repetition_penalty: float | None = None, frequency_penalty: float | None = None,
+             presence_penalty: float | None = None, logit_bias=None, allowed_token_ids=None,
+             grammar=None) -> "TokenRules | None":
+        """Checked rules from a request's fields (ValueError); None when none acts.
+        ``logit_bias``: {token id: value}."""
+        rep = 1.0 if repetition_penalty is None else float(repetition_penalty)
+        freq = 0.0 if frequency_penalty is None else float(frequency_penalty)
+        pres = 0.0 if presence_penalty is None else float(presence_penalty)
+        if not (rep > 0 and math.isfinite(rep)):
+            raise ValueError("repetition_penalty must be > 0")
+        if not (math.isfinite(freq) and math.isfinite(pres)):
+            raise ValueError("frequency_penalty and presence_penalty must be finite")
+        # the rule runs in fp32: what rounds to 0 or infinity there is refused, not applied
+        for name, v in (("repetition_penalty", rep), ("frequency_penalty", freq), ("presence_penalty", pres)):
+            f = float(np.float32(v)) if abs(v) < 3.4e38 else math.inf
+            if not math.isfinite(f) or (v != 0 and f == 0):
+                raise ValueError(f"{name} is outside the range of 32-bit floats")
+        bias = {}
+        for k, v in dict(logit_bias or {}).items():
+            t, b = int(k), float(v)
+            if not 0 <= t < vocab:
+                raise ValueError(f"logit_bias: token {t} is outside the vocabulary of {vocab}")
+            if math.isnan(b) or b > 3.4e38:
+                raise ValueError("logit_bias values must be finite or -inf")
+            if t in bias:
+                raise ValueError(f"logit_bias: token {t} is given twice")
+            bias[t] = b
+        if len(bias) > MAX_BIAS:
+            raise ValueError(f"logit_bias: at most {MAX_BIAS} tokens")
+        if allowed_token_ids is not None:
+            if grammar is not None:
+                raise ValueError("allowed_token_ids and a grammar exclude one another")
+            grammar = AllowedTokens(allowed_token_ids, vocab)
+        if grammar is not None and not callable(getattr(grammar, "mask", None)):
+            raise ValueError("grammar: an object with mask(output) expected")
+        r = TokenRules(rep, freq, pres, tuple(sorted(bias.items())), grammar)
+        return r if r.penalizes or r.bias or r.grammar is not None else None
+
+    def words(self, output, vocab: int, eos_id: int | None) -> np.ndarray | None:
+        """Mask words for the token that follows ``output`` (None: any).  A grammar that
+        allows nothing leaves the end of sequence."""
+        if self.grammar is None:
+            return None
+        w = self.grammar.mask(output)
+        if w is None:
+            return None
+        w = np.ascontiguousarray(w)
+        n = (vocab + 31) // 32
+        if w.ndim != 1 or w.size < n or w.dtype not in (np.int32, np.uint32):
+            raise ValueError(f"grammar mask: {n} int32 words expected")
+        w = w[:n].view(np.int32)
+        if vocab % 32:
+            last = w.view(np.uint32)[-1] & np.uint32((1 << vocab % 32) - 1)
+            if not w[:-1].any() and not last:
+                w = np.zeros(n, np.int32)
+        if not w.any() and eos_id is not None and 0 <= eos_id < vocab:
+            return token_words([eos_id], vocab)
+        return w
 
 
 @dataclass(frozen=True)

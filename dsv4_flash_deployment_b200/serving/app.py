@@ -17,14 +17,17 @@ every reference benchmark sends) is greedy; ``temperature`` > 0 samples
 softmax(logits / T) on the device by the Gumbel-max rule, restricted by
 ``top_k`` (> 0) and ``top_p`` (< 1) when given; ``seed`` makes the samples a
 function of (seed, position) only, so a seeded request repeats its output.
+``repetition_penalty``, ``frequency_penalty``, ``presence_penalty``,
+``logit_bias`` ({token id: value}) and ``allowed_token_ids`` change the logits
+before the token is chosen, greedy or not (models/sampling.py ``TokenRules``).
 ``logprobs`` (completions: the number of alternatives, 0-20; chat:
 ``logprobs: true`` with ``top_logprobs`` 0-20) returns each generated token's
 log-probability under the raw logits and its most likely alternatives, in the
 OpenAI response layouts.  ``n`` choices per prompt (and a list of prompts)
 run as separate engine requests that share the engine's steps; ``best_of``
 is accepted only equal to ``n``.  A request the engine cannot serve is refused
-with 400 (top-k / top-p / logprobs on the tensor-parallel head, logprobs or
-temperature under speculative decoding).
+with 400 (top-k / top-p / logprobs / rules on the tensor-parallel head, logprobs,
+temperature or rules under speculative decoding).
 Streaming sends one SSE event per generated token and ends with
 ``data: [DONE]``; usage rides on the last finish chunk, or with
 ``stream_options: {"include_usage": true}`` in one more chunk with no choices.
@@ -128,11 +131,29 @@ def _params(st: ServerState, body: dict, n_prompt: int, chat: bool = False) -> t
         lp = _logprobs_field(body, chat)
         seed = None if body.get("seed") is None else int(body["seed"])
         sp = SamplingParams(temp, max(top_k, 0), top_p, lp, seed)     # top_k -1 (vLLM's "off") counts as 0
+        rules = _rules_fields(body)
     except (TypeError, ValueError) as e:
         raise web.HTTPBadRequest(text=json.dumps({"error": str(e)}), content_type="application/json") from None
     return (GenParams(mt, bool(body.get("ignore_eos", False)), stop_ids, temp, sp.top_k, sp.top_p, sp.logprobs,
-                      sp.seed),
+                      sp.seed, rules),
             [s for s in stop if s])
+
+
+def _rules_fields(body: dict) -> dict:
+    """Penalties, biases and allowed tokens of a request, the fields that do nothing left
+    out (the engine checks the values)."""
+    out = {}
+    for name, off in (("repetition_penalty", 1.0), ("frequency_penalty", 0.0), ("presence_penalty", 0.0)):
+        if body.get(name) is not None and float(body[name]) != off:
+            out[name] = float(body[name])
+    lb = body.get("logit_bias")
+    if lb:
+        if not isinstance(lb, dict):
+            raise ValueError("logit_bias: an object of token ids and values expected")
+        out["logit_bias"] = {int(k): float(v) for k, v in lb.items()}
+    if body.get("allowed_token_ids") is not None:
+        out["allowed_token_ids"] = [int(t) for t in body["allowed_token_ids"]]
+    return out
 
 
 def _logprobs_field(body: dict, chat: bool) -> int | None:

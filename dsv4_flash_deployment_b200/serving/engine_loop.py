@@ -35,6 +35,8 @@ class GenParams:
     top_p: float = 1.0
     logprobs: int | None = None     # alternatives per token (None: no log-probabilities)
     seed: int | None = None
+    # penalties, logit_bias, allowed_token_ids as the engine's add_request takes them
+    rules: dict = field(default_factory=dict)
 
 
 @dataclass
@@ -146,6 +148,7 @@ class EngineLoop:
                     kw = {}
                     if p.top_k or p.top_p < 1.0 or p.logprobs is not None or p.seed is not None:
                         kw = {"top_k": p.top_k, "top_p": p.top_p, "logprobs": p.logprobs, "seed": p.seed}
+                    kw.update(p.rules)
                     req = eng.add_request(prompt, p.max_tokens, ignore_eos=p.ignore_eos, stop_ids=p.stop_ids,
                                           temperature=p.temperature, **kw)
                 except (ValueError, TypeError) as e:

@@ -20,6 +20,8 @@ def build_local_engine(ec: EngineConfig, ep=None, extra_slots: int = 0, tp=None)
 
     cfg = ec.model_config()
     if ec.device == "cpu":
+        if ec.head_int8:
+            raise ValueError("head_int8 needs a CUDA device")
         from ..io.checkpoint_spec import make_random_weights
         from ..models.oracle_step import OracleStepModel
 
@@ -51,7 +53,7 @@ def build_local_engine(ec: EngineConfig, ep=None, extra_slots: int = 0, tp=None)
                         max_seq_len=ec.max_model_len, weights=weights, seed=ec.seed,
                         expert_storage_layers=storage, ep=ep, use_graphs=ec.use_cuda_graphs,
                         chunk_size=ec.chunk_size, extra_slots=extra_slots, tp=tp, kv_block=ec.kv_block,
-                        kv_pool_tokens=pool, kv_preempt=ec.kv_preempt, engram_shm=ec.engram_shm,
+                        kv_pool_tokens=pool, kv_preempt=ec.kv_preempt, head_int8=ec.head_int8, engram_shm=ec.engram_shm,
                         engram_token_map=_engram_token_map(ec, cfg))
 
 
