@@ -1015,7 +1015,7 @@ size_t i8_stride(const Tensor& t, const char* what) {
 }
 
 void gemm_i8(const Tensor& x, const Tensor& xs, const Tensor& w, const Tensor& ws, const Tensor& out,
-             const Tensor& err) {
+             const Tensor& err, int64_t path, int64_t bn, int64_t splits) {
   CHECK_CUDA(x);
   TORCH_CHECK(x.dim() == 2 && w.dim() == 2, "x: [T, K], w: [N, K]");
   const int64_t T = x.size(0), K = x.size(1), N = w.size(0);
@@ -1028,6 +1028,9 @@ void gemm_i8(const Tensor& x, const Tensor& xs, const Tensor& w, const Tensor& w
   check_vec(ws, "w scale", N, at::kFloat, x);
   check_rows(out, "out", T, N, x);
   const int ot = float_type(out, "out");
+  TORCH_CHECK(path >= 0 && path <= dsv4::I8_PAIRS && (path != dsv4::I8_ROWS || T <= 4) &&
+                  (bn == 0 || bn == 32 || bn == 64 || bn == 128 || bn == 256) && splits >= 0 && splits <= 8,
+              "no such path for these sizes");
   if (T == 0 || N == 0) return;
   dsv4::GemmI8Params p{};
   p.T = (int)T;
@@ -1040,7 +1043,7 @@ void gemm_i8(const Tensor& x, const Tensor& xs, const Tensor& w, const Tensor& w
   p.err = err_word(err, x);
   const c10::cuda::CUDAGuard guard(x.device());
   CUDA_OK(dsv4::gemm_i8(x.data_ptr<int8_t>(), i8_stride(x, "x"), w.data_ptr<int8_t>(), i8_stride(w, "w"), p, ot,
-                        num_sms(), cur_stream()));
+                        (int)path, (int)bn, (int)splits, num_sms(), cur_stream()));
 }
 
 // slots/repetition/frequency/presence/seen/counts together or none; bias_* together or

@@ -95,7 +95,8 @@ bool make_tma_rows_u8(CUtensorMap* map, const void* base, uint64_t rows, uint64_
 // ---------------------------------------------------------- gemm_i8.cu
 struct GemmI8Params {
   int T, N, K;          // tokens, output channels, inner dimension (1 .. 131071)
-  int t_tiles, n_tiles, k_tiles;   // set by gemm_i8
+  int t_tiles, n_tiles, k_tiles, splits;   // set by gemm_i8
+  int width, n_whole, n_units;             // pairs
   const float* xs;      // [T] scale per token
   const float* ws;      // [N] scale per output channel
   void* out;            // [T, N], rows ldo elements apart
@@ -103,8 +104,12 @@ struct GemmI8Params {
   uint32_t* err;
 };
 constexpr int kGemmI8MaxK = 131071;   // 2^14 * 131071 < 2^31: no sum of int8 products passes int32
+// Which kernel runs: chosen by the sizes, or given (tests run each at every size).
+// bn (32, 64, 128, 256) and splits (1..8, at most the k tiles) belong to I8_TILES;
+// 0: the narrowest that holds T up to 256, and 1.
+enum I8Path { I8_AUTO = 0, I8_ROWS = 1 /* T <= 4 */, I8_TILES = 2, I8_PAIRS = 3 };
 // x [T, K], w [N, K]: rows ldx / ldw bytes apart.  otype: FloatType (kernels.h)
-cudaError_t gemm_i8(const int8_t* x, size_t ldx, const int8_t* w, size_t ldw, GemmI8Params p, int otype, int sms,
-                    cudaStream_t st);
+cudaError_t gemm_i8(const int8_t* x, size_t ldx, const int8_t* w, size_t ldw, const GemmI8Params& p, int otype,
+                    int path, int bn, int splits, int sms, cudaStream_t st);
 
 }  // namespace dsv4

@@ -156,8 +156,7 @@ __global__ void __launch_bounds__(kRulesThreads) logits_rules_kernel(LogitsRules
   }
 }
 
-__global__ void history_add_kernel(const int* __restrict__ ids, const int* __restrict__ slots,
-                                   const int* __restrict__ generated, int n, int* seen, int* counts, int n_slots,
+__global__ void history_add_kernel(const int* ids, const int* slots, const int* generated, int n, int* seen, int* counts, int n_slots,
                                    int V, int words, uint32_t* err) {
   pdl_entry();
   const int i = blockIdx.x * blockDim.x + threadIdx.x;

@@ -247,8 +247,8 @@ __global__ void __launch_bounds__(kNormThreads) norm_quant_kernel(NormQuantParam
 
 // y[t, c] = code * scale, rounded to bf16 (8 columns a thread, plain accesses).
 template <int FMT>
-__global__ void dequant_kernel(const uint8_t* __restrict__ q, int ldq, const float* __restrict__ scale,
-                               const uint8_t* __restrict__ sf, int T, int D, __nv_bfloat16* __restrict__ y, int ldy,
+__global__ void dequant_kernel(const uint8_t* q, int ldq, const float* scale, const uint8_t* sf, int T, int D,
+                               __nv_bfloat16* y, int ldy,
                                int vec) {
   pdl_entry();
   const int groups = (D + 7) / 8;

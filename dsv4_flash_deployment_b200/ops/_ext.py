@@ -72,6 +72,7 @@ class _Counting:
                 self.count += n
             return fn(*a, **kw)
 
+        self.__dict__[name] = wrapped     # found directly from the next call on
         return wrapped
 
 

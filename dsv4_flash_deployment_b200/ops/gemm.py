@@ -20,6 +20,7 @@ from . import _ext
 from .layout import ceil_to, expand_block_scales, interleave_w13, sf_to_chunks
 
 KIND_BF16, KIND_MX8, KIND_MX4A = 0, 1, 2
+I8_AUTO, I8_ROWS, I8_TILES, I8_PAIRS = 0, 1, 2, 3
 EPI_BF16, EPI_F32, EPI_SWIGLU = 0, 1, 2
 
 
@@ -27,9 +28,13 @@ class ErrorWord:
     """Per-device int32 error word every kernel may write (0 = healthy)."""
 
     _words: dict = {}
+    _by_device: dict = {}     # by torch.device with an index: the lookup of every call
 
     @classmethod
     def get(cls, device) -> torch.Tensor:
+        w = cls._by_device.get(device)
+        if w is not None:
+            return w
         d = torch.device(device)
         if d.type == "cuda" and d.index is None:   # "cuda" and "cuda:<current>" share one word
             d = torch.device("cuda", torch.cuda.current_device())
@@ -41,7 +46,10 @@ class ErrorWord:
                 mod = _ext.load(required=False)
                 if mod is not None and getattr(mod, "debug_bounds", False):
                     mod.debug_bounds_attach(w)     # index checks of the debug build report here
-        return cls._words[key]
+        w = cls._words[key]
+        if d.type != "cuda" or d.index is not None:
+            cls._by_device[d] = w
+        return w
 
     @classmethod
     def check(cls, device) -> None:
@@ -203,16 +211,19 @@ class I8Weight:
 
 
 def gemm_i8(xq: torch.Tensor, xs: torch.Tensor, w: I8Weight, out: torch.Tensor | None = None,
-            out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+            out_dtype: torch.dtype = torch.bfloat16, path: int = I8_AUTO, bn: int = 0,
+            splits: int = 0) -> torch.Tensor:
     """``out[t, n] = (sum_k xq[t, k] w.q[n, k]) * xs[t] * w.scale[n]``, the sum exact.
 
     ``xq`` int8 [T, K] whose rows start on 16-byte boundaries (as
     :func:`.norm.rms_norm_quant` writes them), ``xs`` fp32 [T]; K up to 131071; out
-    bf16, fp16 or fp32 ``[T, N]`` with contiguous rows."""
+    bf16, fp16 or fp32 ``[T, N]`` with contiguous rows.  ``path``: the kernel chosen
+    by the sizes (``I8_AUTO``) or a given one (csrc/gemm.h, with its token tile ``bn``
+    and K ``splits``); all give the same bits."""
     if out is None:
         out = torch.empty(xq.shape[0], w.q.shape[0], dtype=out_dtype, device=xq.device)
     if xq.is_cuda:
-        _ext.load().gemm_i8(xq, xs, w.q, w.scale, out, ErrorWord.get(xq.device))
+        _ext.load().gemm_i8(xq, xs, w.q, w.scale, out, ErrorWord.get(xq.device), path, bn, splits)
     else:
         if xq.dtype != torch.int8 or xq.shape[1] != w.q.shape[1] or out.shape != (xq.shape[0], w.q.shape[0]):
             raise RuntimeError("int8 x [T, K], w [N, K] and out [T, N] expected")

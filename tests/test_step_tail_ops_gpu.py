@@ -234,6 +234,47 @@ def test_gemm_i8_larger(t, n, k):
         _check_gemm(out, xq, xs, w)
 
 
+@pytest.mark.parametrize("path", [G.I8_ROWS, G.I8_TILES, G.I8_PAIRS])
+@pytest.mark.parametrize("t", [1, 4, 40, 130, 300, 520])
+@pytest.mark.parametrize("n,k", [(1, 1), (129, 33), (640, 4096), (1030, 1279)])
+def test_gemm_i8_every_kernel(t, n, k, path):
+    """Each kernel at sizes that the rule would give to another: the same bits."""
+    xq, xs, w = _i8_case(t, n, k, t + n)
+    if path == G.I8_ROWS and t > 4:
+        with pytest.raises(RuntimeError):
+            G.gemm_i8(xq, xs, w, path=path)
+        return
+    for dt in (BF, F32):
+        out = torch.full((t + 1, n), float("nan"), device="cuda", dtype=dt)
+        G.gemm_i8(xq, xs, w, out[:t], path=path)
+        _done()
+        _check_gemm(out[:t], xq, xs, w)
+        assert torch.isnan(out[t]).all() and torch.equal(out[:t], G.gemm_i8(xq, xs, w, out_dtype=dt))
+
+
+@pytest.mark.parametrize("bn", [32, 64, 128, 256])
+@pytest.mark.parametrize("splits", [1, 2, 3, 5, 8])
+def test_gemm_i8_tile_widths_and_splits(bn, splits):
+    for t, n, k in ((1, 129, 1100), (70, 300, 1279), (290, 513, 4097)):
+        xq, xs, w = _i8_case(t, n, k, t + n)
+        for dt in (BF, F32):
+            out = torch.full((t + 1, n), float("nan"), device="cuda", dtype=dt)
+            G.gemm_i8(xq, xs, w, out[:t], path=G.I8_TILES, bn=bn, splits=splits)
+            _done()
+            _check_gemm(out[:t], xq, xs, w)
+            assert torch.isnan(out[t]).all()
+
+
+def test_gemm_i8_many_tiles_per_block():
+    """More tiles than SMs, in both tensor-core kernels, twice in a row."""
+    xq, xs, w = _i8_case(700, 12000, 640, 1)
+    for path in (G.I8_TILES, G.I8_PAIRS):
+        for _ in range(2):
+            out = G.gemm_i8(xq, xs, w, out_dtype=F32, path=path)
+        _done()
+        _check_gemm(out, xq, xs, w)
+
+
 @pytest.mark.parametrize("t", [1, 3, 40, 300])
 def test_gemm_i8_extreme_codes(t):
     """The largest sums: every product 2^14 over the longest K."""
