@@ -980,7 +980,7 @@ void norm_quant(const Tensor& x, const optional<Tensor>& res, const optional<Ten
   p.q = reinterpret_cast<uint8_t*>(q.data_ptr());
   p.ldq = (size_t)q.stride(0);
   const c10::cuda::CUDAGuard guard(x.device());
-  CUDA_OK(dsv4::norm_quant(p, xt, w ? wt : (xt == dsv4::F_F32 ? dsv4::F_F32 : xt), (int)fmt, cur_stream()));
+  CUDA_OK(dsv4::norm_quant(p, xt, w ? wt : xt, (int)fmt, num_sms(), cur_stream()));
 }
 
 void dequant_rows(const Tensor& q, const Tensor& scale, int64_t fmt, const Tensor& out) {
@@ -998,11 +998,11 @@ void dequant_rows(const Tensor& q, const Tensor& scale, int64_t fmt, const Tenso
   } else {
     check_vec(scale, "scale", q.size(0), at::kFloat, q);
   }
-  TORCH_CHECK(T < (1ll << 31) && D < (1ll << 31) && q.stride(0) < (1ll << 31) && out.stride(0) < (1ll << 31), "too large");
+  TORCH_CHECK(T < (1ll << 31) && D < (1ll << 31), "too large");
   const c10::cuda::CUDAGuard guard(q.device());
-  CUDA_OK(dsv4::dequant_rows(reinterpret_cast<const uint8_t*>(q.data_ptr()), (int)q.stride(0),
+  CUDA_OK(dsv4::dequant_rows(reinterpret_cast<const uint8_t*>(q.data_ptr()), (size_t)q.stride(0),
                              mx ? nullptr : scale.data_ptr<float>(), mx ? scale.data_ptr<uint8_t>() : nullptr, (int)T,
-                             (int)D, (int)fmt, ptr<bf16>(out), (int)out.stride(0), cur_stream()));
+                             (int)D, (int)fmt, ptr<bf16>(out), (size_t)out.stride(0), cur_stream()));
 }
 
 // Row stride of an int8 operand in bytes; TMA wants 16-byte row starts.

@@ -385,7 +385,7 @@ enum FloatType { F_BF16 = 0, F_F16 = 1, F_F32 = 2 };
 // 8-bit row formats: int8 or e4m3 with one fp32 scale per row, MXFP8 (e4m3 with a
 // ue8m0 scale per 32 columns, scale bytes in the GEMM's chunks)
 enum Q8Format { Q8_I8 = 0, Q8_E4M3 = 1, Q8_MX8 = 2 };
-constexpr int kNormMaxD = 32768;   // a row stays in one CTA's registers
+constexpr int kNormMaxD = 32768;   // a row stays in one CTA's registers or shared memory
 struct NormQuantParams {
   int T, D;
   const void* x;         // [T, D], rows ldx apart
@@ -396,14 +396,16 @@ struct NormQuantParams {
   size_t ldro;
   const void* w;         // [D], or null: no norm, only the quantization of x (+ res)
   float eps;
+  double inv_d;          // 1 / D (set by norm_quant)
+  bool aligned;          // every row on 16-byte boundaries (set by norm_quant)
   uint8_t* q;            // [T, D] codes, rows ldq apart
   size_t ldq;
   float* scale;          // [T] (I8, E4M3)
   uint8_t* sf;           // scale chunks (MX8)
 };
-cudaError_t norm_quant(const NormQuantParams& p, int xtype, int wtype, int fmt, cudaStream_t st);
-cudaError_t dequant_rows(const uint8_t* q, int ldq, const float* scale, const uint8_t* sf, int T, int D, int fmt,
-                         __nv_bfloat16* y, int ldy, cudaStream_t st);
+cudaError_t norm_quant(NormQuantParams p, int xtype, int wtype, int fmt, int sms, cudaStream_t st);
+cudaError_t dequant_rows(const uint8_t* q, size_t ldq, const float* scale, const uint8_t* sf, int T, int D, int fmt,
+                         __nv_bfloat16* y, size_t ldy, cudaStream_t st);
 
 // ------------------------------------------------------------ logits.cu
 struct LogitsRules {

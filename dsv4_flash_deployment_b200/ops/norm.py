@@ -19,7 +19,7 @@ from . import _ext
 from .layout import ceil_to, chunks_to_sf, sf_to_chunks
 
 Q8_FMT = {"i8": 0, "e4m3": 1, "mx8": 2}
-MAX_WIDTH = 32768     # a row stays in one thread block's registers
+MAX_WIDTH = 32768     # a row stays in one thread block's registers or shared memory
 
 
 def empty_rows(t: int, d: int, fmt: str, device) -> tuple[torch.Tensor, torch.Tensor]:
