@@ -56,17 +56,21 @@ constexpr int kRulesWords = kRulesCols / 32 + 1;  // bit words that they touch
 constexpr int kRulesChunk = kRulesCols * kRulesThreads / 32;
 
 // Grid (chunks of a row, rows); a warp has 768 columns and works by itself.  Few columns
-// are special (seen before, or biased): they are worked out one lane each, into shared
-// memory, and the pass over all columns only picks them up by a bit.
+// are special (seen before, or biased): they are worked out one lane each, and the pass
+// over all columns knows nothing of them.
 //   1  lane i has word i of the seen bits and of the mask; the logits are asked for
 //   2  the seen columns become a list; a lane per entry reads logit and count and
 //      leaves the penalized value
-//   3  a lane per bias entry adds it to that value or to the logit
-//   4  lane i takes the 16-byte pieces i, i + 32, ..: special values, the mask, store
-// 512 x 129280 fp32 with every rule: 174 us with the counts read in the last pass (four
+//   3  a lane per bias entry adds it to that value, or to the logit and lists the column
+//   4  lane i takes the 16-byte pieces i, i + 32, ..: the mask, store
+//   5  a lane per listed column that the mask allows stores its value over it
+// In place step 4 only touches the pieces that the mask takes something of.
+//
+// 512 x 129280 fp32 with every rule: 174 us with the counts read in step 4 (four
 // dependent reads in a row a piece), 132 us with the steps shared by a block (its
-// barriers), 123 us with 512 columns a warp, 117 us so (569 MB: 4.9 TB/s).  What is left
-// above the copy's 77 us are the dependent reads slot -> bits -> counts.
+// barriers), 117 us with the special values picked up by a bit in step 4 (750
+// instructions a warp), 107 us so (547 MB: 5.1 TB/s).  A copy takes 78 us; the rest are
+// the dependent reads slot -> bits -> counts.
 //
 // A piece starts on a 16-byte boundary whatever the row does, so a row's first and last
 // pieces may be partial; rows of `in` and `out` that start at different offsets from
@@ -78,8 +82,10 @@ __global__ void __launch_bounds__(kRulesThreads) logits_rules_kernel(LogitsRules
   constexpr int P = kRulesCols / (32 * NV);       // pieces of a lane
   constexpr uint32_t kAll = (1u << NV) - 1, kFull = 0xffffffffu;
   __shared__ float s_val[kRulesThreads / 32][kRulesCols];       // values of the special columns
-  __shared__ uint16_t s_list[kRulesThreads / 32][kRulesCols];
-  __shared__ uint32_t s_bits[kRulesThreads / 32][32];
+  __shared__ uint16_t s_list[kRulesThreads / 32][kRulesCols];   // the special columns
+  __shared__ uint32_t s_bits[kRulesThreads / 32][32];           // which they are
+  __shared__ uint32_t s_mask[kRulesThreads / 32][32];
+  __shared__ int s_n[kRulesThreads / 32];
   const int s = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const T* in = static_cast<const T*>(p.in) + (size_t)s * p.ld_in;
   T* out = static_cast<T*>(p.out) + (size_t)s * p.ld_out;
@@ -88,18 +94,6 @@ __global__ void __launch_bounds__(kRulesThreads) logits_rules_kernel(LogitsRules
   const int c0 = ((int)blockIdx.x * (kRulesThreads / 32) + warp) * kRulesCols - shift;   // first column
   if (c0 >= p.V) return;
   const bool inner = vec && c0 >= 0 && c0 + kRulesCols <= p.V;   // every piece is whole
-  float l[P][NV];
-  auto load = [&](int k) {
-    const int v = c0 + (lane + k * 32) * NV;
-    if (inner || (vec && v >= 0 && v + NV <= p.V)) {
-      const Vec<T> q = *reinterpret_cast<const Vec<T>*>(in + v);
-#pragma unroll
-      for (int j = 0; j < NV; ++j) l[k][j] = lg_f(q.v[j]);
-    } else {
-#pragma unroll
-      for (int j = 0; j < NV; ++j) l[k][j] = v + j >= 0 && v + j < p.V ? lg_f(in[v + j]) : 0.f;
-    }
-  };
   // the row's rules; an index outside its table counts as none and is reported
   const int slot = p.slots ? p.slots[s] : -1;
   const int mrow = p.mask ? p.mask_row[s] : -1;
@@ -108,9 +102,24 @@ __global__ void __launch_bounds__(kRulesThreads) logits_rules_kernel(LogitsRules
     b0 = max(0, p.bias_off[s]);
     b1 = min(p.n_bias, p.bias_off[s + 1]);
   }
+  Vec<T> l[P];
   if constexpr (!IN_PLACE) {
+    if (inner) {
 #pragma unroll
-    for (int k = 0; k < P; ++k) load(k);
+      for (int k = 0; k < P; ++k) l[k] = *reinterpret_cast<const Vec<T>*>(in + c0 + (lane + k * 32) * NV);
+    } else {
+#pragma unroll
+      for (int k = 0; k < P; ++k) {
+        const int v = c0 + (lane + k * 32) * NV;
+        if (vec && v >= 0 && v + NV <= p.V) {
+          l[k] = *reinterpret_cast<const Vec<T>*>(in + v);
+        } else {
+#pragma unroll
+          for (int j = 0; j < NV; ++j)
+            if (v + j >= 0 && v + j < p.V) l[k].v[j] = in[v + j];
+        }
+      }
+    }
   }
   bool pen = slot >= 0, masked = mrow >= 0;
   if (slot >= p.n_slots && p.slots) {
@@ -125,26 +134,24 @@ __global__ void __launch_bounds__(kRulesThreads) logits_rules_kernel(LogitsRules
   const int w = wb + lane;
   const bool have = lane < kRulesWords && w >= 0 && w < p.words;
   uint32_t sw = 0, mw = 0;                        // this lane's words: special, allowed
-  float rho = 1.f, freq = 0.f, pres = 0.f;
+  int n = 0;                                      // listed columns
   if (masked && have) mw = (uint32_t)p.mask[(size_t)mrow * p.ld_mask + w];
   if (pen) {
-    rho = p.repetition[s];
-    freq = p.frequency[s];
-    pres = p.presence[s];
+    const float rho = p.repetition[s], freq = p.frequency[s], pres = p.presence[s];
     if (have) sw = (uint32_t)p.seen[(size_t)slot * p.words + w];
     // only the warp's own columns, and none past the vocabulary
     if (lane == 0) sw &= kFull << bit0;
     if (lane == kRulesCols / 32) sw &= (1u << bit0) - 1;
     if (w == p.V >> 5) sw &= (1u << (p.V & 31)) - 1;
     if (rho == 1.f && freq == 0.f && pres == 0.f) sw = 0;
-    int at = __popc(sw);                          // this lane's place in the list
+    if (__any_sync(kFull, sw != 0)) {
+      int at = __popc(sw);                        // this lane's place in the list
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int below = __shfl_up_sync(kFull, at, o);
-      if (lane >= o) at += below;
-    }
-    const int n = __shfl_sync(kFull, at, 31);
-    if (n > 0) {
+      for (int o = 1; o < 32; o <<= 1) {
+        const int below = __shfl_up_sync(kFull, at, o);
+        if (lane >= o) at += below;
+      }
+      n = __shfl_sync(kFull, at, 31);
       at -= __popc(sw);
       for (uint32_t x = sw; x; x &= x - 1) s_list[warp][at++] = (uint16_t)(32 * lane + __ffs(x) - 1 - bit0);
       __syncwarp();
@@ -165,6 +172,7 @@ __global__ void __launch_bounds__(kRulesThreads) logits_rules_kernel(LogitsRules
       b1 = lower_bound(p.bias_id, b0, b1, c0 + kRulesCols);
     }
     s_bits[warp][lane] = sw;
+    if (lane == 0) s_n[warp] = n;
     __syncwarp();
     for (int i = b0 + lane; i < b1; i += 32) {
       const int id = p.bias_id[i], c = id - c0;
@@ -173,51 +181,72 @@ __global__ void __launch_bounds__(kRulesThreads) logits_rules_kernel(LogitsRules
       float b = 0.f;
       for (int j = i; j < b1 && p.bias_id[j] == id; ++j) b += p.bias_val[j];
       const int at = bit0 + c;
-      const bool had = s_bits[warp][at >> 5] >> (at & 31) & 1;   // only this lane sets this bit
+      // the column's bit is asked for and set at once: an id out of its order, and so seen
+      // as another run, adds to what is listed already
+      const bool had = atomicOr(&s_bits[warp][at >> 5], 1u << (at & 31)) >> (at & 31) & 1;
       const float z = had ? s_val[warp][c] : lg_f(in[id]);
       s_val[warp][c] = b == -INFINITY ? b : z + b;
-      if (!had) atomicOr(&s_bits[warp][at >> 5], 1u << (at & 31));
+      if (!had) s_list[warp][atomicAdd(&s_n[warp], 1)] = (uint16_t)c;   // once a column: the list holds them all
     }
     __syncwarp();
-    sw = s_bits[warp][lane];
+    n = s_n[warp];
   }
-  const bool special = __any_sync(kFull, sw != 0);
-#pragma unroll
-  for (int k = 0; k < P; ++k) {
-    const int c = (lane + k * 32) * NV, v = c0 + c;
-    const int i = (bit0 + c) >> 5, sh = (bit0 + c) & 31;
-    uint32_t sp = 0, ok = kAll;
-    if (bit0 == 0) {                              // pieces do not straddle words
-      if (special) sp = __shfl_sync(kFull, sw, i) >> sh & kAll;
-      if (masked) ok = __shfl_sync(kFull, mw, i) >> sh & kAll;
-    } else {
-      if (special) sp = __funnelshift_r(__shfl_sync(kFull, sw, i), __shfl_sync(kFull, sw, i + 1), sh) & kAll;
-      if (masked) ok = __funnelshift_r(__shfl_sync(kFull, mw, i), __shfl_sync(kFull, mw, i + 1), sh) & kAll;
-    }
-    if (!inner && (v + NV <= 0 || v >= p.V)) continue;
-    if constexpr (IN_PLACE) {
-      if (sp == 0 && ok == kAll) continue;
-      if (ok != 0) load(k);                       // nothing of a piece that goes whole is read
-    }
-    if (sp) {
-#pragma unroll
-      for (int j = 0; j < NV; ++j)
-        if (sp >> j & 1) l[k][j] = s_val[warp][c + j];
-    }
+  if constexpr (IN_PLACE) {
     if (masked) {
+      T ninf;
+      lg_set(ninf, -INFINITY);
+      uint32_t ok[P];
 #pragma unroll
-      for (int j = 0; j < NV; ++j)
-        if (!(ok >> j & 1)) l[k][j] = -INFINITY;
+      for (int k = 0; k < P; ++k) {
+        const int c = (lane + k * 32) * NV, v = c0 + c;
+        const int i = (bit0 + c) >> 5, sh = (bit0 + c) & 31;
+        ok[k] = __funnelshift_r(__shfl_sync(kFull, mw, i), __shfl_sync(kFull, mw, i + 1), sh) & kAll;
+        // nothing of a piece that stays or goes whole is read
+        if (ok[k] != 0 && ok[k] != kAll && v >= 0 && v + NV <= p.V) l[k] = *reinterpret_cast<const Vec<T>*>(in + v);
+      }
+#pragma unroll
+      for (int k = 0; k < P; ++k) {
+        const int v = c0 + (lane + k * 32) * NV;
+        if (ok[k] == kAll) continue;
+        if (v >= 0 && v + NV <= p.V) {
+#pragma unroll
+          for (int j = 0; j < NV; ++j)
+            if (!(ok[k] >> j & 1)) l[k].v[j] = ninf;
+          *reinterpret_cast<Vec<T>*>(out + v) = l[k];
+        } else {
+#pragma unroll
+          for (int j = 0; j < NV; ++j)
+            if (!(ok[k] >> j & 1) && v + j >= 0 && v + j < p.V) out[v + j] = ninf;
+        }
+      }
     }
-    if (inner || (vec && v >= 0 && v + NV <= p.V)) {
-      Vec<T> q;
+  } else {
 #pragma unroll
-      for (int j = 0; j < NV; ++j) lg_set(q.v[j], l[k][j]);
-      *reinterpret_cast<Vec<T>*>(out + v) = q;
-    } else {
+    for (int k = 0; k < P; ++k) {
+      const int c = (lane + k * 32) * NV, v = c0 + c;
+      if (masked) {
+        const int i = (bit0 + c) >> 5, sh = (bit0 + c) & 31;
+        uint32_t ok = __shfl_sync(kFull, mw, i) >> sh;
+        if (bit0 != 0) ok = __funnelshift_r(__shfl_sync(kFull, mw, i), __shfl_sync(kFull, mw, i + 1), sh);   // a piece may straddle words
 #pragma unroll
-      for (int j = 0; j < NV; ++j)
-        if (v + j >= 0 && v + j < p.V) lg_set(out[v + j], l[k][j]);
+        for (int j = 0; j < NV; ++j)
+          if (!(ok >> j & 1)) lg_set(l[k].v[j], -INFINITY);
+      }
+      if (inner || (vec && v >= 0 && v + NV <= p.V)) {
+        *reinterpret_cast<Vec<T>*>(out + v) = l[k];
+      } else {
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+          if (v + j >= 0 && v + j < p.V) out[v + j] = l[k].v[j];
+      }
+    }
+  }
+  if (n > 0) {
+    if (masked) s_mask[warp][lane] = mw;
+    __syncwarp();   // also: these stores come after the lanes' stores to the same places
+    for (int i = lane; i < n; i += 32) {
+      const int c = s_list[warp][i], at = bit0 + c;
+      if (!masked || (s_mask[warp][at >> 5] >> (at & 31) & 1)) lg_set(out[c0 + c], s_val[warp][c]);
     }
   }
 }
