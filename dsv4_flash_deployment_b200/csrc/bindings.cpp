@@ -920,6 +920,13 @@ void check_vec(const Tensor& t, const char* what, int64_t n, at::ScalarType ty, 
               str(t.sizes()), " on ", str(t.device()));
 }
 
+void check_chunks(const Tensor& t, int64_t rows, int64_t cols, const Tensor& like) {
+  TORCH_CHECK(t.device() == like.device() && t.scalar_type() == at::kByte && t.is_contiguous() && t.dim() == 3 &&
+                  t.size(0) >= (rows + 127) / 128 && t.size(1) == cols / 128 && t.size(2) == 512,
+              "scale: uint8 chunks [>= ", str((rows + 127) / 128), ", ", str(cols / 128), ", 512] expected, got ",
+              str(t.sizes()));
+}
+
 uint32_t* err_word(const Tensor& err, const Tensor& like) {
   TORCH_CHECK(err.device() == like.device() && err.scalar_type() == at::kInt && err.numel() >= 1, "error word");
   return reinterpret_cast<uint32_t*>(err.data_ptr<int>());
@@ -932,8 +939,8 @@ void norm_quant(const Tensor& x, const optional<Tensor>& res, const optional<Ten
   CHECK_CUDA(x);
   TORCH_CHECK(x.dim() == 2 && (x.stride(1) == 1 || x.size(1) <= 1), "x: [T, D] with contiguous rows");
   const int64_t T = x.size(0), D = x.size(1);
-  TORCH_CHECK(D <= dsv4::kNormMaxD, "width ", str(D), ": at most ", str(dsv4::kNormMaxD));
-  TORCH_CHECK(T < (1ll << 31), "too many rows");
+  TORCH_CHECK(D >= 1 && D <= dsv4::kNormMaxD, "width ", str(D), ": 1 to ", str(dsv4::kNormMaxD));
+  TORCH_CHECK(T < (1ll << 31) - 65536, "too many rows");
   const int xt = float_type(x, "x");
   dsv4::NormQuantParams p{};
   p.T = (int)T;
@@ -968,9 +975,7 @@ void norm_quant(const Tensor& x, const optional<Tensor>& res, const optional<Ten
   if (fmt == dsv4::Q8_MX8) {
     TORCH_CHECK(D % 128 == 0, "MXFP8 rows: width must be a multiple of 128");
     TORCH_CHECK(q.dim() == 2 && q.size(0) >= T && q.size(1) == D && q.is_contiguous(), "q: contiguous [>= T, D]");
-    TORCH_CHECK(scale.device() == x.device() && scale.scalar_type() == at::kByte && scale.is_contiguous() &&
-                    scale.numel() >= (T + 127) / 128 * (D / 128) * 512,
-                "scale: uint8 chunks [ceil(T / 128), D / 128, 512]");
+    check_chunks(scale, T, D, x);
     p.sf = scale.data_ptr<uint8_t>();
   } else {
     check_rows(q, "q", T, D, x);
@@ -992,9 +997,8 @@ void dequant_rows(const Tensor& q, const Tensor& scale, int64_t fmt, const Tenso
   check_rows(out, "out", T, D, q);
   const bool mx = fmt == dsv4::Q8_MX8;
   if (mx) {
-    TORCH_CHECK(D % 128 == 0 && scale.device() == q.device() && scale.scalar_type() == at::kByte &&
-                    scale.is_contiguous() && scale.numel() >= (T + 127) / 128 * (D / 128) * 512,
-                "scale: uint8 chunks [ceil(T / 128), D / 128, 512]");
+    TORCH_CHECK(D % 128 == 0, "MXFP8 rows: width must be a multiple of 128");
+    check_chunks(scale, T, D, q);
   } else {
     check_vec(scale, "scale", q.size(0), at::kFloat, q);
   }
@@ -1028,7 +1032,7 @@ void gemm_i8(const Tensor& x, const Tensor& xs, const Tensor& w, const Tensor& w
   check_vec(ws, "w scale", N, at::kFloat, x);
   check_rows(out, "out", T, N, x);
   const int ot = float_type(out, "out");
-  TORCH_CHECK(path >= 0 && path <= dsv4::I8_PAIRS && (path != dsv4::I8_ROWS || T <= 4) &&
+  TORCH_CHECK(path >= 0 && path <= dsv4::I8_PAIRS && (path != dsv4::I8_ROWS || T <= 2) &&
                   (bn == 0 || bn == 32 || bn == 64 || bn == 128 || bn == 256) && splits >= 0 && splits <= 8,
               "no such path for these sizes");
   if (T == 0 || N == 0) return;

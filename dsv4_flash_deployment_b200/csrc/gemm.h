@@ -107,7 +107,7 @@ constexpr int kGemmI8MaxK = 131071;   // 2^14 * 131071 < 2^31: no sum of int8 pr
 // Which kernel runs: chosen by the sizes, or given (tests run each at every size).
 // bn (32, 64, 128, 256) and splits (1..8, at most the k tiles) belong to I8_TILES;
 // 0: the narrowest that holds T up to 256, and 1.
-enum I8Path { I8_AUTO = 0, I8_ROWS = 1 /* T <= 4 */, I8_TILES = 2, I8_PAIRS = 3 };
+enum I8Path { I8_AUTO = 0, I8_ROWS = 1 /* T <= 2 */, I8_TILES = 2, I8_PAIRS = 3 };
 // x [T, K], w [N, K]: rows ldx / ldw bytes apart.  otype: FloatType (kernels.h)
 cudaError_t gemm_i8(const int8_t* x, size_t ldx, const int8_t* w, size_t ldw, const GemmI8Params& p, int otype,
                     int path, int bn, int splits, int sms, cudaStream_t st);

@@ -8,7 +8,7 @@
 // result, however K is split.
 //
 // Three kernels; gemm_i8() at the end chooses by the sizes:
-//   rows   T <= 4: a warp per few weight rows, dp4a.  Bound by the weight's bytes.
+//   rows   T <= 2: a warp per few weight rows, dp4a.  Bound by the weight's bytes.
 //   tiles  tcgen05.mma kind::i8, one SM per 128 x BN tile, K split over a cluster
 //          where the tiles are fewer than the SMs.
 //   pairs  tcgen05.mma with cta_group::2, two SMs per 256 x 256 tile.
@@ -315,7 +315,7 @@ done:
   }
 }
 
-// ------------------------------------------------------------- T <= 4: rows
+// ------------------------------------------------------------- T <= 2: rows
 // A warp takes R weight rows and all T tokens; lane l reads the 16-byte pieces l,
 // l + 32, .. of a row, the tokens' pieces from L1/L2 beside it, four dp4a a piece
 // and token, and the lanes' sums meet in one integer warp reduction.
@@ -335,7 +335,7 @@ __global__ void __launch_bounds__(256) gemm_i8_rows_kernel(const int8_t* x, size
 #pragma unroll
     for (int t = 0; t < T; ++t) acc[r][t] = 0;
   const int full = p.K / 512 * 512;
-  constexpr int kUnroll = R == 1 ? 8 : R == 2 ? 4 : 2;
+  constexpr int kUnroll = R == 1 ? 8 : 2;
 #pragma unroll kUnroll
   for (int k = 16 * lane; k < full; k += 512) {
     int4 a[R], b[T];
@@ -613,7 +613,7 @@ cudaError_t launch_rows(const int8_t* x, size_t ldx, const int8_t* w, size_t ldw
     const unsigned grid = (unsigned)((p.N + 8 * rows - 1) / (8 * rows));
     return launch_pdl(kernel, grid, 256, 0, st, x, ldx, w, ldw, p);
   };
-  if (p.N >= 4 * 32 * sms) return go(gemm_i8_rows_kernel<T, T <= 2 ? 4 : 2, TO>, T <= 2 ? 4 : 2);
+  if (p.N >= 4 * 32 * sms) return go(gemm_i8_rows_kernel<T, 4, TO>, 4);
   return go(gemm_i8_rows_kernel<T, 1, TO>, 1);
 }
 
@@ -734,8 +734,6 @@ cudaError_t run_i8(const int8_t* x, size_t ldx, const int8_t* w, size_t ldw, Gem
     switch (p.T) {
       case 1: return launch_rows<1, TO>(x, ldx, w, ldw, p, sms, st);
       case 2: return launch_rows<2, TO>(x, ldx, w, ldw, p, sms, st);
-      case 3: return launch_rows<3, TO>(x, ldx, w, ldw, p, sms, st);
-      case 4: return launch_rows<4, TO>(x, ldx, w, ldw, p, sms, st);
       default: return cudaErrorInvalidValue;
     }
   }

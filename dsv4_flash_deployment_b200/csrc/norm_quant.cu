@@ -159,8 +159,14 @@ DSV4_DEV uint32_t codes4(F2 a, F2 b, float k) {
     return lo | hi << 16;
   }
 }
-DSV4_DEV float abs_max(float m, F2 a) { return fmaxf(m, fmaxf(fabsf(a.x), fabsf(a.y))); }
-// Largest of the warp's values, none negative: their bits order as they do.
+// NaN wins, so that a NaN weight shows in the maximum as a NaN in the row does in the sum.
+DSV4_DEV float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+DSV4_DEV float abs_max(float m, F2 a) { return max_nan(m, max_nan(fabsf(a.x), fabsf(a.y))); }
+// Largest of the warp's values, none negative: their bits order as they do (NaN on top).
 DSV4_DEV float warp_max_abs(float v) { return __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(v))); }
 
 // What takes s w to its code: r * top / max|y|, with max|y| = r * max|s w| kept above
@@ -338,7 +344,7 @@ __global__ void __launch_bounds__(WARP ? 128 : kNormThreads) norm_quant_kernel(N
           float s = c < D ? row_again<TX>(p, ro, t, c) * kDown : 0.f;
           part += s * s;
           if (c < D && !kMx) s *= to_f(static_cast<const TW*>(p.w)[c]);
-          mx = fmaxf(mx, fabsf(s));
+          mx = max_nan(mx, fabsf(s));
           (j & 1 ? v[k][j >> 1].y : v[k][j >> 1].x) = s;
         }
       if constexpr (!WARP) __syncthreads();   // red is still being read
@@ -462,7 +468,7 @@ __global__ void __launch_bounds__(kNormThreads) norm_quant_staged_kernel(NormQua
       if (ro) ro[c] = from_f<TX>(s);
       part += s * s;
       const float sw = w && !kMx ? s * to_f(wc[i]) : s;
-      mx = fmaxf(mx, fabsf(sw));
+      mx = max_nan(mx, fabsf(sw));
       s_row[c] = sw;
     }
   }
@@ -483,7 +489,7 @@ __global__ void __launch_bounds__(kNormThreads) norm_quant_staged_kernel(NormQua
       const float s = row_again<TX>(p, ro, t, c) * kDown;
       part += s * s;
       s_row[c] = kMx ? s : s * to_f(w[c]);
-      mx = fmaxf(mx, fabsf(s_row[c]));
+      mx = max_nan(mx, fabsf(s_row[c]));
     }
     ss = part;
     row_sum_max<false, Sum>(ss, mx, red[1]);

@@ -35,6 +35,8 @@ class TokenHistory:
                    torch.zeros(n_slots, vocab, dtype=torch.int32, device=device))
 
     def reset(self, slot: int) -> None:
+        if not 0 <= slot < len(self.counts):
+            raise IndexError(f"slot {slot} of {len(self.counts)}")
         self.seen[slot].zero_()
         self.counts[slot].zero_()
 
@@ -94,7 +96,9 @@ class RowRules:
 def apply_logits_rules(logits: torch.Tensor, rules: RowRules, history: TokenHistory | None = None,
                        out: torch.Tensor | None = None) -> torch.Tensor:
     """Applies ``rules`` to ``logits`` [S, V] (bf16, fp16 or fp32, contiguous rows) into
-    ``out`` (None: in place) and returns it.  ``history`` is needed with penalties."""
+    ``out`` (None: in place; else it may not overlap the logits) and returns it.
+    ``history`` is needed with penalties.  A slot or mask row outside its table leaves
+    the row without that rule and is reported in the device error word."""
     r = rules
     if r.slots is not None and history is None:
         raise ValueError("penalties need a token history")

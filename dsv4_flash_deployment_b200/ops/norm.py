@@ -38,13 +38,14 @@ def rms_norm_quant(x: torch.Tensor, weight: torch.Tensor, eps: float, fmt: str =
                    q_out: torch.Tensor | None = None, scale_out: torch.Tensor | None = None):
     """``y = rmsnorm(x + residual) * weight`` in fp32, quantized to ``fmt``.
 
-    ``x`` [T, D] bf16, fp16 or fp32 with contiguous rows (any row stride), D up to
+    ``x`` [T, D] bf16, fp16 or fp32 with contiguous rows (any row stride), D from 1 to
     32768 (``"mx8"``: a multiple of 128); ``residual`` of x's type; ``weight`` [D] of
     x's type or fp32; ``eps`` at least 1e-30.  Returns ``(q, scale)``, or with a
     residual ``(q, scale, residual_out)`` with the sum rounded to x's type
     (``residual_out`` may be ``residual`` or ``x`` itself; the norm takes the sum
     before its rounding).  ``q_out`` / ``scale_out``: buffers to write
-    (:func:`empty_rows`).  Rows that hold an infinity or NaN come out as NaN (their
+    (:func:`empty_rows`); apart from ``residual_out`` being an input whole, no output
+    may overlap an input.  Rows that hold an infinity or NaN come out as NaN (their
     scale is NaN)."""
     f = Q8_FMT.get(fmt)
     if f is None:
@@ -108,8 +109,8 @@ def dequantize_rows(q: torch.Tensor, scale: torch.Tensor, rows: int | None = Non
 def _cpu(x, residual, residual_out, weight, eps, fmt, q_out, scale_out) -> None:
     """The operator on CPU tensors, with the device binding's checks."""
     t, d = x.shape
-    if d > MAX_WIDTH:
-        raise RuntimeError(f"width {d}: at most {MAX_WIDTH}")
+    if not 1 <= d <= MAX_WIDTH:
+        raise RuntimeError(f"width {d}: 1 to {MAX_WIDTH}")
     if weight is not None and eps < 1e-30:
         raise RuntimeError("eps must be at least 1e-30")
     if weight is not None and (weight.shape != (d,) or weight.dtype not in (x.dtype, torch.float32)):

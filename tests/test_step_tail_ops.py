@@ -116,6 +116,9 @@ def test_history_counts_prompt_and_output():
         h.add(i([70]), i([0]), i([1]))
     h.reset(0)
     assert not h.seen.any() and not h.counts.any()
+    for slot in (-1, 2):
+        with pytest.raises(IndexError):
+            h.reset(slot)
 
 
 def test_rules_cpu_against_the_formula():

@@ -183,11 +183,34 @@ def test_norm_refusals_on_the_device():
            dict(residual=x.half()), dict(residual=x[:1]), dict(residual_out=x.clone()),
            dict(q_out=torch.zeros(2, 64, device="cuda")), dict(scale_out=torch.zeros(3, device="cuda")),
            dict(residual=torch.ones(1, 64, device="cuda").expand(2, 64)), dict(x=x.double()), dict(x=x.t()),
-           dict(x=torch.ones(1, 32776, device="cuda"), weight=torch.ones(32776, device="cuda"))]
+           dict(x=torch.ones(1, 32776, device="cuda"), weight=torch.ones(32776, device="cuda")),
+           dict(x=x[:, :0], weight=w[:0])]
     for b in bad:
         kw = dict(dict(x=x, weight=w, eps=1e-6), **b)
         with pytest.raises(RuntimeError):
             Q.rms_norm_quant(**kw)
+    _done()
+
+
+def test_norm_weights_that_are_not_finite():
+    x = torch.randn(3, 256, device="cuda")
+    for bad in (float("nan"), float("inf")):
+        w = torch.ones(256, device="cuda")
+        w[17] = bad
+        for xx in (x, x[:, :255]):      # aligned and odd rows
+            q, s = Q.rms_norm_quant(xx, w[: xx.shape[1]].contiguous(), 1e-6)
+            assert torch.isnan(s).all() and not q.any()
+    _done()
+
+
+def test_norm_wrong_scale_chunks_are_refused():
+    x = torch.ones(3, 256, device="cuda")
+    q = torch.empty(128, 256, device="cuda", dtype=torch.uint8)
+    for shape in ((1, 1, 512), (1, 4, 512), (1024,), (0, 2, 512)):
+        with pytest.raises(RuntimeError):
+            Q.quantize_rows(x, "mx8", q_out=q, scale_out=torch.empty(shape, device="cuda", dtype=torch.uint8))
+        with pytest.raises(RuntimeError):
+            Q.dequantize_rows(q, torch.empty(shape, device="cuda", dtype=torch.uint8), 3)
     _done()
 
 
@@ -235,12 +258,12 @@ def test_gemm_i8_larger(t, n, k):
 
 
 @pytest.mark.parametrize("path", [G.I8_ROWS, G.I8_TILES, G.I8_PAIRS])
-@pytest.mark.parametrize("t", [1, 4, 40, 130, 300, 520])
-@pytest.mark.parametrize("n,k", [(1, 1), (129, 33), (640, 4096), (1030, 1279)])
+@pytest.mark.parametrize("t", [1, 2, 3, 40, 130, 300, 520])
+@pytest.mark.parametrize("n,k", [(1, 1), (129, 33), (640, 4096), (1030, 1279), (20000, 520)])
 def test_gemm_i8_every_kernel(t, n, k, path):
     """Each kernel at sizes that the rule would give to another: the same bits."""
     xq, xs, w = _i8_case(t, n, k, t + n)
-    if path == G.I8_ROWS and t > 4:
+    if path == G.I8_ROWS and t > 2:
         with pytest.raises(RuntimeError):
             G.gemm_i8(xq, xs, w, path=path)
         return
@@ -507,6 +530,36 @@ def test_rules_refusals_on_the_device():
             h.add(*a)
     assert L.apply_logits_rules(lg[:0], L.RowRules()).shape == (0, 64)
     _done()
+
+
+# ------------------------------------------------------- offsets past 32 bits
+def test_offsets_past_32_bits():
+    """The last rows of arrays with more than 2^31 elements."""
+    t, d = 270000, 8192
+    x = torch.zeros(t, d, device="cuda", dtype=BF)
+    x[-3:] = torch.randn(3, d, device="cuda", generator=_gen(1)).to(BF)
+    w = torch.ones(d, device="cuda", dtype=BF)
+    q, s = Q.rms_norm_quant(x, w, 1e-6)
+    _done()
+    _check_norm((q[-3:], s[-3:].contiguous()), x[-3:], w, 1e-6, "i8", None)
+    wt = G.I8Weight(torch.ones(16, d, device="cuda", dtype=torch.int8), torch.ones(16, device="cuda"))
+    out = G.gemm_i8(q, s, wt, out_dtype=F32)
+    _done()
+    _check_gemm(out[-3:], q[-3:], s[-3:], wt)
+    y = Q.dequantize_rows(q, s)
+    assert torch.equal(y[-3:], (q[-3:].float() * s[-3:, None]).to(BF))
+    del x, q, y, out
+    n = 129280
+    xq, xs, wn = _i8_case(17000, n, 64, 2)
+    out = G.gemm_i8(xq, xs, wn)
+    _done()
+    _check_gemm(out[-40:], xq[-40:], xs[-40:], wn)
+    keep = out[-2:].clone()
+    bits = torch.rand(1, n, device="cuda", generator=_gen(3)) < 0.5
+    r = L.RowRules().masks(torch.zeros(17000, device="cuda", dtype=torch.int32), N.pack_bits(bits))
+    L.apply_logits_rules(out, r)
+    _done()
+    assert torch.equal(out[-2:], torch.where(bits, keep, torch.full_like(keep, float("-inf"))))
 
 
 # ---------------------------------------------------------------- all of them
