@@ -397,7 +397,6 @@ struct NormQuantParams {
   const void* w;         // [D], or null: no norm, only the quantization of x (+ res)
   float eps;
   double inv_d;          // 1 / D (set by norm_quant)
-  bool aligned;          // every row on 16-byte boundaries (set by norm_quant)
   uint8_t* q;            // [T, D] codes, rows ldq apart
   size_t ldq;
   float* scale;          // [T] (I8, E4M3)

@@ -395,9 +395,11 @@ __global__ void __launch_bounds__(WARP ? 128 : kNormThreads) norm_quant_kernel(N
 
 // Every other row: any alignment, any width up to 32768.  A block per row, which waits in
 // shared memory (as s w in fp32; MX8: as s) between the two halves; off 16-byte
-// boundaries element accesses, neighbours in a warp, eight in flight a thread.
-template <typename TX, typename TW, int FMT>
-__global__ void __launch_bounds__(kNormThreads) norm_quant_staged_kernel(NormQuantParams p) {
+// boundaries element accesses, neighbours in a warp, eight in flight a thread (777 x 5003
+// fp32: 9.8 us, with four 11.0; in 16-byte pieces from the boundary before the row 13.2,
+// since a lane's columns then lie apart in the weights and in shared memory).
+template <typename TX, typename TW, int FMT, bool ALIGNED>
+__global__ void __launch_bounds__(kNormThreads, 2) norm_quant_staged_kernel(NormQuantParams p) {
   pdl_entry();
   extern __shared__ __align__(16) float s_row[];   // D, rounded up to 4
   constexpr bool kMx = FMT == Q8_MX8;
@@ -409,7 +411,7 @@ __global__ void __launch_bounds__(kNormThreads) norm_quant_staged_kernel(NormQua
   TX* ro = p.res_out ? static_cast<TX*>(p.res_out) + (size_t)t * p.ldro : nullptr;
   const TW* w = static_cast<const TW*>(p.w);
   float part = 0.f, mx = 0.f;
-  if (p.aligned) {   // wide rows on 16-byte boundaries: two groups of 8 columns in flight
+  if constexpr (ALIGNED) {   // wide rows on 16-byte boundaries: two groups of 8 columns in flight
     for (int g0 = tid; g0 < D / 8; g0 += 2 * nt) {
       Vec8<TX> a[2], b[2];
       Vec8<TW> wc[2];
@@ -447,29 +449,30 @@ __global__ void __launch_bounds__(kNormThreads) norm_quant_staged_kernel(NormQua
         *reinterpret_cast<float4*>(s_row + c + 4) = make_float4(v[2].x, v[2].y, v[3].x, v[3].y);
       }
     }
-  }
-  constexpr int U = 8;
-  for (int c0 = p.aligned ? D : tid; c0 < D; c0 += U * nt) {
-    TX a[U], b[U];
-    TW wc[U];
+  } else {
+    constexpr int U = 8;
+    for (int c0 = tid; c0 < D; c0 += U * nt) {
+      TX a[U], b[U];
+      TW wc[U];
 #pragma unroll
-    for (int i = 0; i < U; ++i) {
-      const int c = min(c0 + i * nt, D - 1);   // past the end: not used
-      a[i] = x[c];
-      if (res) b[i] = res[c];
-      if (w && !kMx) wc[i] = w[c];
-    }
+      for (int i = 0; i < U; ++i) {
+        const int c = min(c0 + i * nt, D - 1);   // past the end: not used
+        a[i] = x[c];
+        if (res) b[i] = res[c];
+        if (w && !kMx) wc[i] = w[c];
+      }
 #pragma unroll
-    for (int i = 0; i < U; ++i) {
-      const int c = c0 + i * nt;
-      if (c >= D) break;
-      float s = to_f(a[i]);
-      if (res) s += to_f(b[i]);
-      if (ro) ro[c] = from_f<TX>(s);
-      part += s * s;
-      const float sw = w && !kMx ? s * to_f(wc[i]) : s;
-      mx = max_nan(mx, fabsf(sw));
-      s_row[c] = sw;
+      for (int i = 0; i < U; ++i) {
+        const int c = c0 + i * nt;
+        if (c >= D) break;
+        float s = to_f(a[i]);
+        if (res) s += to_f(b[i]);
+        if (ro) ro[c] = from_f<TX>(s);
+        part += s * s;
+        const float sw = w && !kMx ? s * to_f(wc[i]) : s;
+        mx = max_nan(mx, fabsf(sw));
+        s_row[c] = sw;
+      }
     }
   }
   if (tid < (4 - D % 4) % 4) s_row[D + tid] = 0.f;
@@ -582,17 +585,19 @@ __global__ void __launch_bounds__(256) dequant_kernel(const uint8_t* q, size_t l
 
 // ------------------------------------------------------------------- host
 template <typename TX, typename TW, int FMT>
-static cudaError_t launch_norm(NormQuantParams p, bool vec, int sms, cudaStream_t st) {
+static cudaError_t launch_norm(const NormQuantParams& p, bool vec, int sms, cudaStream_t st) {
   if (!vec || p.D > 2 * 8 * kNormThreads) {
-    static std::atomic<uint64_t> configured{0};
-    const cudaError_t e = smem_attr_once(norm_quant_staged_kernel<TX, TW, FMT>, 4 * kNormMaxD, configured);
-    if (e != cudaSuccess) return e;
-    p.aligned = vec;
     // 8 columns a thread while the rows leave SMs idle, 16 once they come in waves
     const int each = p.T <= 2 * sms ? 8 : 16;
     const int nt = std::min(kNormThreads, std::max(32, (p.D / each + 31) / 32 * 32));
-    return launch_pdl(norm_quant_staged_kernel<TX, TW, FMT>, (unsigned)p.T, (unsigned)nt, (size_t)(p.D + 3) / 4 * 16, st,
-                      p);
+    auto go = [&](auto kernel, std::atomic<uint64_t>& configured) {
+      const cudaError_t e = smem_attr_once(kernel, 4 * kNormMaxD, configured);
+      if (e != cudaSuccess) return e;
+      return launch_pdl(kernel, (unsigned)p.T, (unsigned)nt, (size_t)(p.D + 3) / 4 * 16, st, p);
+    };
+    static std::atomic<uint64_t> aligned{0}, any{0};
+    return vec ? go(norm_quant_staged_kernel<TX, TW, FMT, true>, aligned)
+               : go(norm_quant_staged_kernel<TX, TW, FMT, false>, any);
   }
   // as many blocks as are resident at once, each with its share of the rows
   auto go = [&](auto kernel, int nt, int rows_per_block, std::atomic<int>* room) {
