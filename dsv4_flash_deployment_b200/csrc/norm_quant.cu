@@ -184,7 +184,7 @@ DSV4_DEV float code_scale(float r, float mx, float top, float* up) {
 
 // Sum and maximum over the threads of a row, in a fixed order: the result does not
 // depend on which warp arrives first.  One barrier; the caller alternates `red`.
-// MXFP8 sums in 64 bits past the thread's own part (see norm_once).
+// MXFP8 sums in 64 bits (see norm_once).
 template <typename Sum>
 struct RowRed {
   Sum sum[32];
@@ -232,12 +232,31 @@ DSV4_DEV Root inv_root(double sum, const NormQuantParams& p, float eps) {
   r.lo = c - (r.hi - r0);
   return r;
 }
-// s * w * r rounded once.  MXFP8 scales are powers of two, so y's own rounding errors
-// are all that moves a code to its neighbour; with three roundings in a row that was
-// about one code in a million, with this one in seven million.
-DSV4_DEV float norm_once(float s, float w, Root r) {
-  const float v = s * w;
-  return fmaf(v, r.hi, fmaf(fmaf(s, w, -v), r.hi, v * r.lo));
+DSV4_DEV void add_squares(F2 a, double& x, double& y) {
+  x = fma((double)a.x, (double)a.x, x);
+  y = fma((double)a.y, (double)a.y, y);
+}
+
+// y = s * w * r rounded once, for MXFP8: its scales are powers of two, so y's own rounding
+// errors are all that moves a code to its neighbour (one code in a million with three
+// roundings in a row and the sum in 32 bits).  Rounded once, y can only mislead the code
+// where it lies exactly between two codes, and so has its low 19 bits zero; there it is
+// rounded to odd instead (to the neighbour with an odd last bit where it is not exact),
+// and rounding that to a code is rounding the product itself.
+DSV4_DEV F2 norm_once(F2 s, F2 w, Root r) {
+  const F2 v = mul2(s, w), ev{fmaf(s.x, w.x, -v.x), fmaf(s.y, w.y, -v.y)};   // s w = v + ev
+  return fma2(v, {r.hi, r.hi}, fma2(ev, {r.hi, r.hi}, mul2(v, {r.lo, r.lo})));
+}
+DSV4_DEV bool between_codes(F2 y) {
+  return (__float_as_uint(y.x) & 0x7ffffu) == 0 || (__float_as_uint(y.y) & 0x7ffffu) == 0;
+}
+DSV4_DEV float norm_odd(float s, float w, Root r) {
+  const float v = s * w, ev = fmaf(s, w, -v);
+  const float y0 = v * r.hi, e0 = fmaf(v, r.hi, -y0);      // v r.hi = y0 + e0
+  const float c = fmaf(ev, r.hi, v * r.lo) + e0, y = y0 + c, rest = c - (y - y0);
+  uint32_t b = __float_as_uint(y);
+  if (rest != 0.f && !(b & 1u)) b += (__float_as_uint(rest) ^ b) >> 31 ? 0xffffffffu : 1u;
+  return __uint_as_float(b);
 }
 
 }  // namespace
@@ -291,6 +310,7 @@ __global__ void __launch_bounds__(WARP ? 128 : kNormThreads) norm_quant_kernel(N
   for (int t = row0; t < p.T; t += rows, turn ^= 1) {
     TX* ro = p.res_out ? static_cast<TX*>(p.res_out) + (size_t)t * p.ldro : nullptr;
     F2 v[PER][4], sq{0.f, 0.f};
+    double dx = 0.0, dy = 0.0;
     float mx = 0.f;
 #pragma unroll
     for (int k = 0; k < PER; ++k) {
@@ -310,8 +330,13 @@ __global__ void __launch_bounds__(WARP ? 128 : kNormThreads) norm_quant_kernel(N
     if (t + rows < p.T) fetch(t + rows);
 #pragma unroll
     for (int k = 0; k < PER; ++k) {
+      if constexpr (kMx) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) sq = fma2(v[k][j], v[k][j], sq);
+        for (int j = 0; j < 4; ++j) add_squares(v[k][j], dx, dy);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) sq = fma2(v[k][j], v[k][j], sq);
+      }
       if (!kMx && has_w && col(k) < D) {
         F2 f[4];
         floats_of(wv[k], f);
@@ -321,18 +346,17 @@ __global__ void __launch_bounds__(WARP ? 128 : kNormThreads) norm_quant_kernel(N
 #pragma unroll
       for (int j = 0; j < 4; ++j) mx = abs_max(mx, v[k][j]);
     }
-    float part = sq.x + sq.y;
-    Sum ss = part;
+    Sum ss = kMx ? Sum(dx + dy) : Sum(sq.x + sq.y);
     row_sum_max<WARP, Sum>(ss, mx, red[turn]);
     bool bad;
     Root r{1.f, 0.f};
     if (!has_w) {
       bad = ss != ss || !(mx < INFINITY);   // no norm: squares may overflow, infinities and NaN may not pass
-    } else if (ss < INFINITY && mx < INFINITY) {
+    } else if ((float)ss < INFINITY && mx < INFINITY) {
       bad = false;
       r = inv_root(ss, p, p.eps);
     } else {   // all threads of the row alike: the row again, scaled by 2^-96
-      part = 0.f;
+      ss = 0;
       mx = 0.f;
 #pragma unroll
       for (int k = 0; k < PER; ++k)
@@ -342,15 +366,14 @@ __global__ void __launch_bounds__(WARP ? 128 : kNormThreads) norm_quant_kernel(N
           // residual_out may be the residual itself and then holds the rounded sum: the
           // ratio of two such rows differs by that rounding only
           float s = c < D ? row_again<TX>(p, ro, t, c) * kDown : 0.f;
-          part += s * s;
+          ss += (Sum)s * (Sum)s;
           if (c < D && !kMx) s *= to_f(static_cast<const TW*>(p.w)[c]);
           mx = max_nan(mx, fabsf(s));
           (j & 1 ? v[k][j >> 1].y : v[k][j >> 1].x) = s;
         }
       if constexpr (!WARP) __syncthreads();   // red is still being read
-      ss = part;
       row_sum_max<WARP, Sum>(ss, mx, red[turn]);
-      bad = !(ss < INFINITY) || !(mx < INFINITY);
+      bad = !((float)ss < INFINITY) || !(mx < INFINITY);
       if (!bad) r = inv_root(ss, p, 0.f);
     }
     uint8_t* q = p.q + (size_t)t * p.ldq;
@@ -375,7 +398,10 @@ __global__ void __launch_bounds__(WARP ? 128 : kNormThreads) norm_quant_kernel(N
           floats_of(wv[k], f);   // past the row's end: not used, v is 0 there
 #pragma unroll
           for (int j = 0; j < 4; ++j)
-            v[k][j] = c < D ? F2{norm_once(v[k][j].x, f[j].x, r), norm_once(v[k][j].y, f[j].y, r)} : F2{0.f, 0.f};
+            if (c < D) {
+              const F2 y = norm_once(v[k][j], f[j], r);
+              v[k][j] = between_codes(y) ? F2{norm_odd(v[k][j].x, f[j].x, r), norm_odd(v[k][j].y, f[j].y, r)} : y;
+            }
         }
         float am = 0.f;
 #pragma unroll
@@ -410,7 +436,8 @@ __global__ void __launch_bounds__(kNormThreads, 2) norm_quant_staged_kernel(Norm
   const TX* res = p.res ? static_cast<const TX*>(p.res) + (size_t)t * p.ldr : nullptr;
   TX* ro = p.res_out ? static_cast<TX*>(p.res_out) + (size_t)t * p.ldro : nullptr;
   const TW* w = static_cast<const TW*>(p.w);
-  float part = 0.f, mx = 0.f;
+  Sum ss = 0;
+  float mx = 0.f;
   if constexpr (ALIGNED) {   // wide rows on 16-byte boundaries: two groups of 8 columns in flight
     for (int g0 = tid; g0 < D / 8; g0 += 2 * nt) {
       Vec8<TX> a[2], b[2];
@@ -434,10 +461,17 @@ __global__ void __launch_bounds__(kNormThreads, 2) norm_quant_staged_kernel(Norm
           for (int j = 0; j < 4; ++j) v[j] = add2(v[j], f[j]);
         }
         if (ro) st_vec8(ro + c, v);
-        F2 sq{0.f, 0.f};
+        if constexpr (kMx) {
+          double dx = 0.0, dy = 0.0;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) sq = fma2(v[j], v[j], sq);
-        part += sq.x + sq.y;
+          for (int j = 0; j < 4; ++j) add_squares(v[j], dx, dy);
+          ss += dx + dy;
+        } else {
+          F2 sq{0.f, 0.f};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) sq = fma2(v[j], v[j], sq);
+          ss += sq.x + sq.y;
+        }
         if (w && !kMx) {
           floats_of(wc[i], f);
 #pragma unroll
@@ -468,7 +502,7 @@ __global__ void __launch_bounds__(kNormThreads, 2) norm_quant_staged_kernel(Norm
         float s = to_f(a[i]);
         if (res) s += to_f(b[i]);
         if (ro) ro[c] = from_f<TX>(s);
-        part += s * s;
+        ss += (Sum)s * (Sum)s;
         const float sw = w && !kMx ? s * to_f(wc[i]) : s;
         mx = max_nan(mx, fabsf(sw));
         s_row[c] = sw;
@@ -476,27 +510,25 @@ __global__ void __launch_bounds__(kNormThreads, 2) norm_quant_staged_kernel(Norm
     }
   }
   if (tid < (4 - D % 4) % 4) s_row[D + tid] = 0.f;
-  Sum ss = part;
   row_sum_max<false, Sum>(ss, mx, red[0]);
   bool bad;
   Root r{1.f, 0.f};
   if (!w) {
     bad = ss != ss || !(mx < INFINITY);
-  } else if (ss < INFINITY && mx < INFINITY) {
+  } else if ((float)ss < INFINITY && mx < INFINITY) {
     bad = false;
     r = inv_root(ss, p, p.eps);
   } else {
-    part = 0.f;
+    ss = 0;
     mx = 0.f;
     for (int c = tid; c < D; c += nt) {
       const float s = row_again<TX>(p, ro, t, c) * kDown;
-      part += s * s;
+      ss += (Sum)s * (Sum)s;
       s_row[c] = kMx ? s : s * to_f(w[c]);
       mx = max_nan(mx, fabsf(s_row[c]));
     }
-    ss = part;
     row_sum_max<false, Sum>(ss, mx, red[1]);
-    bad = !(ss < INFINITY) || !(mx < INFINITY);
+    bad = !((float)ss < INFINITY) || !(mx < INFINITY);
     if (!bad) r = inv_root(ss, p, 0.f);
   }
   __syncthreads();   // the row is complete (a block of one warp has met no barrier yet)
@@ -514,7 +546,7 @@ __global__ void __launch_bounds__(kNormThreads, 2) norm_quant_staged_kernel(Norm
     if constexpr (kMx) {                        // 8 lanes hold a block of 32 columns
       if (w)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) y[j] = norm_once(y[j], to_f(w[c + j]), r);
+        for (int j = 0; j < 4; ++j) y[j] = norm_odd(y[j], to_f(w[c + j]), r);
       float am = fmaxf(fmaxf(fabsf(y[0]), fabsf(y[1])), fmaxf(fabsf(y[2]), fabsf(y[3])));
 #pragma unroll
       for (int o = 1; o < 8; o <<= 1) am = fmaxf(am, __shfl_xor_sync(0xffffffffu, am, o));
