@@ -21,7 +21,7 @@
 //
 // Warp roles (320 threads): warp 0 TMA producer, warp 1 TMEM owner and MMA issuer,
 // warps 2..9 epilogue, two per TMEM lane quadrant, which take a tile's 32-token
-// chunks in turn (with one per quadrant a pair's last tile ended 4 us later).
+// chunks in turn: a tile's epilogue has to fit beside the products of the next.
 // Persistent over output tiles; two accumulators in TMEM, so the epilogue of a tile
 // overlaps the products of the next.
 #include <cuda_fp16.h>
@@ -112,10 +112,9 @@ DSV4_DEV int split_begin(int k_tiles, int splits, int i) { return (int)((long lo
 
 // One 32-token column chunk of a tile: the integer sums of this lane's channel,
 // scaled and stored (32 lanes write 32 neighbouring channels of a token).  The
-// tokens' scales come from shared memory, four to a broadcast read: a shuffle per
-// token takes as much of the shared-memory path as the store itself, which the
-// tensor core's operand reads need (tile of 256 x 256, K 4096, fp32: 22.2 -> 20.6 k
-// cycles).  Whole chunks go without a test per store (those took 4 times as long).
+// tokens' scales come from shared memory, four to a broadcast read (a shuffle per token
+// instead: 12 k cycles a 256 x 256 fp32 tile against 11 k).  Whole chunks go without a
+// test per store: with one a bf16 tile's epilogue took 13.5 k cycles, now 6.5 k.
 template <typename TO>
 DSV4_DEV void store_chunk(const uint32_t (&r)[32], int nt, const float4* xs, float ws, TO* out, size_t ldo, bool live) {
   float v[32];
@@ -190,8 +189,7 @@ __global__ void __launch_bounds__(kI8Threads, 1)
   // Work unit -> (channel tile, token tile, split).  Token tiles of one channel tile
   // are next to each other: CTAs that run together share the weight tile in L2.  With
   // splits > 1 a unit is one CTA (no loop) and the splits of a tile are one cluster.
-  // One lane alone runs the producer's and the issuer's loop: a warp barrier per k tile
-  // costs the tensor core more than the k tile's last instruction hides.
+  // One lane alone runs the producer's and the issuer's loop: no warp barrier per k tile.
   if (warp == 0) {
     if (lane == 0) {
       int stage = 0;
@@ -318,7 +316,10 @@ done:
 // ------------------------------------------------------------- T <= 2: rows
 // A warp takes R weight rows and all T tokens; lane l reads the 16-byte pieces l,
 // l + 32, .. of a row, the tokens' pieces from L1/L2 beside it, four dp4a a piece
-// and token, and the lanes' sums meet in one integer warp reduction.
+// and token, and the lanes' sums meet in one integer warp reduction.  Four rows a warp
+// where the rows fill the SMs several times, else one, for more loads in flight.
+// One token, 129280 x 4096: 80 us (6.6 TB/s; the tensor-core tiles 83); 1280 x 5120:
+// 3.5 us (tiles 5.0, of which most is getting started: barriers, TMEM, the first TMA).
 template <int T, int R, typename TO>
 __global__ void __launch_bounds__(256) gemm_i8_rows_kernel(const int8_t* x, size_t ldx, const int8_t* w, size_t ldw,
                                                            GemmI8Params p) {
@@ -376,6 +377,12 @@ __global__ void __launch_bounds__(256) gemm_i8_rows_kernel(const int8_t* x, size
 // shared memory, and each CTA's TMEM gets its 128 channels x all 256 tokens.  Per
 // product that is a third less L2 -> SM traffic than a CTA of its own with a 128 x
 // 256 tile moves, which is what bounds the latter.
+// Measured in the kernel: 598 cycles a k tile (512 would be the tensor core's own; the
+// reads of both operands and the TMA writes share the shared-memory path), 675 with
+// fp32 stores beside it; a warp barrier in the issuing loop made the first 619.
+// 8192^3: 380 us, 2.9 POP/s (tiles 430 us); 4096 x 5120 x 8192: 120 us (tiles 127 us,
+// and 164 us before its epilogue).  Run for seconds the GPU is at its power cap, 1.3 to
+// 1.5 GHz, and the same products take 10 to 25 % longer.
 constexpr int kPairStages = 6;
 constexpr int kPairA = 128 * 128, kPairB = 128 * 128, kPairStage = kPairA + kPairB;
 constexpr int kPairSmem = 1024 + kPairStages * kPairStage + kEpiWarps * 128 * 4 + 256;
@@ -693,7 +700,11 @@ int cluster_room_bn(int bn, int splits) {
 // tensor core's 0.35 us a k tile), so a choice costs, in 128-byte rows loaded by the
 // busiest SM (640 to a microsecond): the rows of its k tiles, 6 a token column for
 // the epilogue, and with K split 768 for the cluster's barriers and 7 a column to
-// park and add the partial tiles.
+// park and add the partial tiles.  Against every width and split timed at 17 shapes
+// from 3 x 2560 x 5120 to 2048 x 2048 x 4096 the choice was the fastest or within 4 %
+// of it at 15 (64 x 2304 x 1280: 5.6 us, the widest tile with K in 4 parts 18.5), 13 %
+// off at 1500 x 700 x 7000 and a third at 256 x 1280 x 5120 (14.9 us; 256-token tiles
+// with K in 8 parts 11.1).
 struct I8Plan {
   int path, bn, splits;
 };
