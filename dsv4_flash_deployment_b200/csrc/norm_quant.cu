@@ -423,15 +423,20 @@ __global__ void __launch_bounds__(WARP ? 128 : kNormThreads) norm_quant_kernel(N
 // shared memory (as s w in fp32; MX8: as s) between the two halves; off 16-byte
 // boundaries element accesses, neighbours in a warp, eight in flight a thread (777 x 5003
 // fp32: 9.8 us, with four 11.0; in 16-byte pieces from the boundary before the row 13.2,
-// since a lane's columns then lie apart in the weights and in shared memory).
-template <typename TX, typename TW, int FMT, bool ALIGNED>
+// since a lane's columns then lie apart in the weights and in shared memory).  WARP: a
+// warp per row, 8 rows a block.
+constexpr int kStagedWarps = 8;
+template <typename TX, typename TW, int FMT, bool ALIGNED, bool WARP>
 __global__ void __launch_bounds__(kNormThreads, 2) norm_quant_staged_kernel(NormQuantParams p) {
   pdl_entry();
-  extern __shared__ __align__(16) float s_row[];   // D, rounded up to 4
+  extern __shared__ __align__(16) float s_rows[];   // a row: D, rounded up to 4
   constexpr bool kMx = FMT == Q8_MX8;
   using Sum = typename std::conditional<kMx, double, float>::type;
   __shared__ RowRed<Sum> red[2];
-  const int tid = threadIdx.x, nt = blockDim.x, t = blockIdx.x, D = p.D;
+  const int tid = WARP ? threadIdx.x & 31 : threadIdx.x, nt = WARP ? 32 : blockDim.x, D = p.D;
+  const int t = WARP ? (int)blockIdx.x * kStagedWarps + (int)(threadIdx.x >> 5) : (int)blockIdx.x;
+  if (WARP && t >= p.T) return;   // a warp alike; no barrier of the block follows
+  float* s_row = s_rows + (WARP ? (size_t)(threadIdx.x >> 5) * ((D + 3) / 4 * 4) : 0);
   const TX* x = static_cast<const TX*>(p.x) + (size_t)t * p.ldx;
   const TX* res = p.res ? static_cast<const TX*>(p.res) + (size_t)t * p.ldr : nullptr;
   TX* ro = p.res_out ? static_cast<TX*>(p.res_out) + (size_t)t * p.ldro : nullptr;
@@ -510,7 +515,7 @@ __global__ void __launch_bounds__(kNormThreads, 2) norm_quant_staged_kernel(Norm
     }
   }
   if (tid < (4 - D % 4) % 4) s_row[D + tid] = 0.f;
-  row_sum_max<false, Sum>(ss, mx, red[0]);
+  row_sum_max<WARP, Sum>(ss, mx, red[0]);
   bool bad;
   Root r{1.f, 0.f};
   if (!w) {
@@ -527,11 +532,14 @@ __global__ void __launch_bounds__(kNormThreads, 2) norm_quant_staged_kernel(Norm
       s_row[c] = kMx ? s : s * to_f(w[c]);
       mx = max_nan(mx, fabsf(s_row[c]));
     }
-    row_sum_max<false, Sum>(ss, mx, red[1]);
+    row_sum_max<WARP, Sum>(ss, mx, red[1]);
     bad = !((float)ss < INFINITY) || !(mx < INFINITY);
     if (!bad) r = inv_root(ss, p, 0.f);
   }
-  __syncthreads();   // the row is complete (a block of one warp has met no barrier yet)
+  if constexpr (WARP)   // the row is complete
+    __syncwarp();
+  else
+    __syncthreads();   // (a block of one warp has met no barrier yet)
   uint8_t* q = p.q + (size_t)t * p.ldq;
   const bool words = reinterpret_cast<uintptr_t>(q) % 4 == 0;
   constexpr float top = FMT == Q8_I8 ? 127.f : 448.f;
@@ -602,6 +610,24 @@ __global__ void __launch_bounds__(256) dequant_kernel(const uint8_t* q, size_t l
     st_vec8(y + (size_t)t * ldy + c, v[0]);
     st_vec8(y + (size_t)t * ldy + c + 8, v[1]);
   } else {
+    if (per_row == 0) {   // narrow rows: 8 of all elements in order, 256 apart
+      const unsigned long long n = (unsigned long long)T * D, i0 = (unsigned long long)blockIdx.x * 2048 + threadIdx.x;
+      int t[8], c[8];
+      uint8_t b[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const unsigned long long i = i0 + 256 * j < n ? i0 + 256 * j : n - 1;   // past the end: not used
+        t[j] = (int)(i >> 32 ? i / (unsigned)D : (unsigned)i / (unsigned)D);
+        c[j] = (int)(i - (unsigned long long)t[j] * D);
+        b[j] = q[(size_t)t[j] * ldq + c[j]];
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (i0 + 256 * j < n)
+          y[(size_t)t[j] * ldy + c[j]] =
+              __float2bfloat16(code_value<FMT>(b[j]) * dequant_scale<FMT>(scale, sf, t[j], c[j], D / 128));
+      return;
+    }
     const int t = (int)(blockIdx.x / per_row), c0 = (int)(blockIdx.x % per_row) * 2048 + (int)threadIdx.x;
     const uint8_t* src = q + (size_t)t * ldq;
     uint8_t b[8];
@@ -622,14 +648,20 @@ static cudaError_t launch_norm(const NormQuantParams& p, bool vec, int sms, cuda
     // 8 columns a thread while the rows leave SMs idle, 16 once they come in waves
     const int each = p.T <= 2 * sms ? 8 : 16;
     const int nt = std::min(kNormThreads, std::max(32, (p.D / each + 31) / 32 * 32));
+    const size_t row_bytes = (size_t)(p.D + 3) / 4 * 16;
+    // very many narrow rows: a warp each (9135 x 37 fp16: 9.9 us with a block a row, 5.2 so;
+    // x 1001 bf16: 21.8 and 20.4; 1200 x 1001: 6.2 and 6.6)
+    if (!vec && p.D <= 1024 && p.T >= 16 * sms)
+      return launch_pdl(norm_quant_staged_kernel<TX, TW, FMT, false, true>, (unsigned)((p.T + kStagedWarps - 1) / kStagedWarps),
+                        32 * kStagedWarps, kStagedWarps * row_bytes, st, p);
     auto go = [&](auto kernel, std::atomic<uint64_t>& configured) {
       const cudaError_t e = smem_attr_once(kernel, 4 * kNormMaxD, configured);
       if (e != cudaSuccess) return e;
-      return launch_pdl(kernel, (unsigned)p.T, (unsigned)nt, (size_t)(p.D + 3) / 4 * 16, st, p);
+      return launch_pdl(kernel, (unsigned)p.T, (unsigned)nt, row_bytes, st, p);
     };
     static std::atomic<uint64_t> aligned{0}, any{0};
-    return vec ? go(norm_quant_staged_kernel<TX, TW, FMT, true>, aligned)
-               : go(norm_quant_staged_kernel<TX, TW, FMT, false>, any);
+    return vec ? go(norm_quant_staged_kernel<TX, TW, FMT, true, false>, aligned)
+               : go(norm_quant_staged_kernel<TX, TW, FMT, false, false>, any);
   }
   // as many blocks as are resident at once, each with its share of the rows
   auto go = [&](auto kernel, int nt, int rows_per_block, std::atomic<int>* room) {
@@ -700,9 +732,14 @@ static cudaError_t launch_dequant(const uint8_t* q, size_t ldq, const float* sca
                                   __nv_bfloat16* y, size_t ldy, cudaStream_t st) {
   const bool vec = D % 16 == 0 && ldq % 16 == 0 && ldy % 8 == 0 && reinterpret_cast<uintptr_t>(q) % 16 == 0 &&
                    reinterpret_cast<uintptr_t>(y) % 16 == 0;
-  const unsigned per_row = vec ? (unsigned)(D / 16) : (unsigned)((D + 2047) / 2048);
-  const unsigned long long blocks =
-      vec ? ((unsigned long long)T * per_row + 255) / 256 : (unsigned long long)T * per_row;
+  // A block for 2048 columns of a row, or for 2048 elements of many narrow rows, where a
+  // division each costs less than idle threads (9135 x 37: 12.7 us and 4.0; x 401: 13.6
+  // and 10.4; x 1001: 19.5 and 24.1; 300 x 37: 1.6 and 3.1)
+  const bool flat = D <= 512 && T >= 4096;
+  const unsigned per_row = vec ? (unsigned)(D / 16) : flat ? 0u : (unsigned)((D + 2047) / 2048);
+  const unsigned long long blocks = vec    ? ((unsigned long long)T * per_row + 255) / 256
+                                    : flat ? ((unsigned long long)T * D + 2047) / 2048
+                                           : (unsigned long long)T * per_row;
   if (blocks >= (1ull << 31)) return cudaErrorInvalidValue;
   if (vec)
     launch_pdl(dequant_kernel<FMT, true>, (unsigned)blocks, 256, 0, st, q, ldq, scale, sf, T, D, y, ldy, per_row);

@@ -97,6 +97,29 @@ def test_norm_widths(t, d, fmt):
 
 
 @pytest.mark.parametrize("fmt", ["i8", "e4m3", "mx8"])
+@pytest.mark.parametrize("t,d,off", [(5003, 37, 0), (4097, 256, 1), (2500, 511, 0), (2369, 1024, 3), (1300, 256, 0),
+                                     (2369, 512, 0), (1201, 1024, 0), (1200, 1536, 0)])
+@pytest.mark.parametrize("dt,wt", [(BF, BF), (F32, F32)])
+def test_norm_many_narrow_rows(t, d, off, dt, wt, fmt):
+    """Rows that a warp each takes, on 16-byte boundaries and off them; two of them are not finite."""
+    if fmt == "mx8" and d % 128:
+        d = 128
+    g = _gen(t + d)
+    x = torch.randn(t, d + 8, device="cuda", generator=g).to(dt)[:, off:off + d]
+    res = (2 * torch.randn(t, d, device="cuda", generator=g)).to(dt)
+    w = (1 + 0.2 * torch.randn(d, device="cuda", generator=g)).to(wt)
+    got = Q.rms_norm_quant(x, w, 1e-6, fmt, residual=res)
+    _done()
+    _check_norm(got, x, w, 1e-6, fmt, res)
+    x[t - 1, d - 1], x[t // 2, 0] = float("nan"), float("inf")
+    again = Q.rms_norm_quant(x, w, 1e-6, fmt, residual=res)
+    v, want = (Q.dequantize_rows(*r[:2], t) for r in (again, got))
+    _done()
+    want[[t - 1, t // 2]] = float("nan")
+    assert torch.equal(v.isnan(), want.isnan()) and torch.equal(v.nan_to_num(), want.nan_to_num())
+
+
+@pytest.mark.parametrize("fmt", ["i8", "e4m3", "mx8"])
 @pytest.mark.parametrize("dt,wt", [(BF, BF), (BF, F32), (HF, HF), (HF, F32), (F32, F32)])
 @pytest.mark.parametrize("res", [False, True])
 def test_norm_types_strides_and_offsets(dt, wt, fmt, res):
