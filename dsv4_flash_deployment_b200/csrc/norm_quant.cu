@@ -28,7 +28,7 @@
 
 namespace dsv4 {
 
-constexpr int kNormThreads = 512;
+constexpr int kNormThreads = 512, kNormWide = 768;
 
 namespace {
 
@@ -182,8 +182,8 @@ DSV4_DEV float code_scale(float r, float mx, float top, float* up) {
   return r * inv;
 }
 
-// Sum and maximum over the threads of a row, in a fixed order: the result does not
-// depend on which warp arrives first.  One barrier; the caller alternates `red`.
+// Sum and maximum over the threads of a row (at most MAXT), in a fixed order: the result
+// does not depend on which warp arrives first.  One barrier; the caller alternates `red`.
 // MXFP8 sums in 64 bits (see norm_once).
 template <typename Sum>
 struct RowRed {
@@ -195,7 +195,7 @@ DSV4_DEV double warp_sum(double v) {
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
-template <bool WARP, typename Sum>
+template <bool WARP, int MAXT, typename Sum>
 DSV4_DEV void row_sum_max(Sum& sum, float& mx, RowRed<Sum>& red) {
   sum = warp_sum(sum);
   mx = warp_max_abs(mx);
@@ -209,7 +209,7 @@ DSV4_DEV void row_sum_max(Sum& sum, float& mx, RowRed<Sum>& red) {
   __syncthreads();
   sum = lane < nw ? red.sum[lane] : Sum(0);
 #pragma unroll
-  for (int o = kNormThreads / 64; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  for (int o = MAXT / 32 > 16 ? 16 : 8; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   sum = __shfl_sync(0xffffffffu, sum, 0);
   mx = warp_max_abs(lane < nw ? red.mx[lane] : 0.f);
 }
@@ -278,8 +278,8 @@ DSV4_DEV float mx_inv(uint32_t e, bool bad) { return bad ? 0.f : exp_to_f32(254 
 // int8, 470 MB: 118 us with a block per row (load, reduce and store in turn, 2 blocks
 // an SM), 88 us with single fp32 operations (273 instructions for a lane's 8 columns:
 // issue slots), 82 us so (5.7 TB/s).
-template <typename TX, typename TW, int FMT, bool WARP, int PER>
-__global__ void __launch_bounds__(WARP ? 128 : kNormThreads) norm_quant_kernel(NormQuantParams p) {
+template <typename TX, typename TW, int FMT, bool WARP, int PER, int MAXT, int MINB>
+__global__ void __launch_bounds__(MAXT, MINB) norm_quant_kernel(NormQuantParams p) {
   pdl_entry();
   const int tid = WARP ? threadIdx.x & 31 : threadIdx.x, nt = WARP ? 32 : blockDim.x;
   const int row0 = WARP ? (int)(blockIdx.x * 4 + (threadIdx.x >> 5)) : (int)blockIdx.x;
@@ -347,7 +347,7 @@ __global__ void __launch_bounds__(WARP ? 128 : kNormThreads) norm_quant_kernel(N
       for (int j = 0; j < 4; ++j) mx = abs_max(mx, v[k][j]);
     }
     Sum ss = kMx ? Sum(dx + dy) : Sum(sq.x + sq.y);
-    row_sum_max<WARP, Sum>(ss, mx, red[turn]);
+    row_sum_max<WARP, MAXT>(ss, mx, red[turn]);
     bool bad;
     Root r{1.f, 0.f};
     if (!has_w) {
@@ -372,7 +372,7 @@ __global__ void __launch_bounds__(WARP ? 128 : kNormThreads) norm_quant_kernel(N
           (j & 1 ? v[k][j >> 1].y : v[k][j >> 1].x) = s;
         }
       if constexpr (!WARP) __syncthreads();   // red is still being read
-      row_sum_max<WARP, Sum>(ss, mx, red[turn]);
+      row_sum_max<WARP, MAXT>(ss, mx, red[turn]);
       bad = !((float)ss < INFINITY) || !(mx < INFINITY);
       if (!bad) r = inv_root(ss, p, 0.f);
     }
@@ -515,7 +515,7 @@ __global__ void __launch_bounds__(kNormThreads, 2) norm_quant_staged_kernel(Norm
     }
   }
   if (tid < (4 - D % 4) % 4) s_row[D + tid] = 0.f;
-  row_sum_max<WARP, Sum>(ss, mx, red[0]);
+  row_sum_max<WARP, kNormThreads>(ss, mx, red[0]);
   bool bad;
   Root r{1.f, 0.f};
   if (!w) {
@@ -532,7 +532,7 @@ __global__ void __launch_bounds__(kNormThreads, 2) norm_quant_staged_kernel(Norm
       s_row[c] = kMx ? s : s * to_f(w[c]);
       mx = max_nan(mx, fabsf(s_row[c]));
     }
-    row_sum_max<WARP, Sum>(ss, mx, red[1]);
+    row_sum_max<WARP, kNormThreads>(ss, mx, red[1]);
     bad = !((float)ss < INFINITY) || !(mx < INFINITY);
     if (!bad) r = inv_root(ss, p, 0.f);
   }
@@ -677,24 +677,33 @@ static cudaError_t launch_norm(const NormQuantParams& p, bool vec, int sms, cuda
     const int turns = (want + per_sm * sms - 1) / (per_sm * sms);
     return launch_pdl(kernel, (unsigned)((want + turns - 1) / turns), (unsigned)nt, 0, st, p);
   };
-#define DSV4_NQ(W, P, NT, ROWS)                                             \
-  do {                                                                      \
-    static std::atomic<int> room[kNormThreads / 32 + 1] = {};               \
-    return go(norm_quant_kernel<TX, TW, FMT, W, P>, NT, ROWS, room);        \
+#define DSV4_NQ(W, P, NT, ROWS, MAXT, MINB)                                    \
+  do {                                                                         \
+    static std::atomic<int> room[kNormWide / 32 + 1] = {};                     \
+    return go(norm_quant_kernel<TX, TW, FMT, W, P, MAXT, MINB>, NT, ROWS, room); \
   } while (0)
   const int groups = p.D / 8;
   // many narrow rows: a warp each (4096 x 1280 bf16: 8.5 us with a block a row, 6.8 us so)
   constexpr int kWarpGroups = sizeof(TX) == 2 ? 192 : 64;   // what a lane's registers hold
   if (groups <= kWarpGroups && p.T >= 8 * sms) {
-    if (groups <= 32) DSV4_NQ(true, 1, 128, 4);
-    if (groups <= 64) DSV4_NQ(true, 2, 128, 4);
+    if (groups <= 32) DSV4_NQ(true, 1, 128, 4, 128, 1);
+    if (groups <= 64) DSV4_NQ(true, 2, 128, 4, 128, 1);
     if constexpr (sizeof(TX) == 2) {
-      if (groups <= 128) DSV4_NQ(true, 4, 128, 4);
-      DSV4_NQ(true, 6, 128, 4);
+      if (groups <= 128) DSV4_NQ(true, 4, 128, 4, 128, 1);
+      DSV4_NQ(true, 6, 128, 4, 128, 1);
     }
   }
-  if (groups <= kNormThreads) DSV4_NQ(false, 1, (groups + 31) / 32 * 32, 1);
-  DSV4_NQ(false, 2, ((groups + 1) / 2 + 31) / 32 * 32, 1);
+  // 16-bit rows: two blocks of 512 threads an SM (64 registers; 16384 x 4096 bf16 to MXFP8
+  // 108 us, with one block an SM 139), and one group a thread up to 6144 columns (512 x 5120
+  // to MXFP8 7.8 us, with two groups a thread 8.8; to int8 5.9 and 6.1)
+  const int nt1 = (groups + 31) / 32 * 32;
+  if constexpr (sizeof(TX) == 2) {
+    if (groups <= kNormThreads) DSV4_NQ(false, 1, nt1, 1, kNormThreads, 2);
+    if (groups <= kNormWide) DSV4_NQ(false, 1, nt1, 1, kNormWide, 1);
+  } else {
+    if (groups <= kNormThreads) DSV4_NQ(false, 1, nt1, 1, kNormThreads, 1);
+  }
+  DSV4_NQ(false, 2, ((groups + 1) / 2 + 31) / 32 * 32, 1, kNormThreads, 1);
 #undef DSV4_NQ
 }
 

@@ -82,7 +82,8 @@ def _check_norm(got, x, w, eps, fmt, res):
 
 @pytest.mark.parametrize("fmt", ["i8", "e4m3", "mx8"])
 @pytest.mark.parametrize("t,d", [(1, 1), (2, 8), (1, 4096), (3, 33), (7, 128), (130, 1024), (5, 5003), (300, 5120),
-                                 (9, 8200), (2, 16384), (2, 32768), (3, 32767)])
+                                 (300, 4224), (5, 6144), (5, 6272), (300, 8192), (9, 8200), (2, 16384), (2, 32768),
+                                 (3, 32767)])
 def test_norm_widths(t, d, fmt):
     if fmt == "mx8" and d % 128:
         d = -(-d // 128) * 128
