@@ -574,7 +574,8 @@ __global__ void __launch_bounds__(kNormThreads, 2) norm_quant_staged_kernel(Norm
 }
 
 // y[t, c] = code * scale, rounded to bf16.  A thread has 16 columns of a row next to each
-// other (VEC: 16-byte accesses), or 8 that are 256 apart.
+// other (16-byte accesses), or 8 elements that are 256 apart, of a row or of all rows in
+// order.
 template <int FMT>
 DSV4_DEV float dequant_scale(const float* scale, const uint8_t* sf, int t, int c, int k_tiles) {
   if constexpr (FMT == Q8_MX8) {
@@ -589,11 +590,12 @@ DSV4_DEV float code_value(uint8_t b) {
   return FMT == Q8_I8 ? (float)(int8_t)b : e4m3_to_f32(b);
 }
 
-template <int FMT, bool VEC>
+enum DequantWalk { DQ_VEC, DQ_ROW, DQ_FLAT };
+template <int FMT, DequantWalk WALK>
 __global__ void __launch_bounds__(256) dequant_kernel(const uint8_t* q, size_t ldq, const float* scale, const uint8_t* sf,
                                                       int T, int D, __nv_bfloat16* y, size_t ldy, unsigned per_row) {
   pdl_entry();
-  if constexpr (VEC) {
+  if constexpr (WALK == DQ_VEC) {
     const unsigned long long gid = (unsigned long long)blockIdx.x * 256 + threadIdx.x;   // per_row = D / 16
     const unsigned hi = (unsigned)(gid >> 32);
     const int t = hi ? (int)(gid / per_row) : (int)((unsigned)gid / per_row);
@@ -609,25 +611,23 @@ __global__ void __launch_bounds__(256) dequant_kernel(const uint8_t* q, size_t l
                                  code_value<FMT>((uint8_t)(w[j >> 2] >> (8 * (j & 3) + 8))) * s};
     st_vec8(y + (size_t)t * ldy + c, v[0]);
     st_vec8(y + (size_t)t * ldy + c + 8, v[1]);
-  } else {
-    if (per_row == 0) {   // narrow rows: 8 of all elements in order, 256 apart
-      const unsigned long long n = (unsigned long long)T * D, i0 = (unsigned long long)blockIdx.x * 2048 + threadIdx.x;
-      int t[8], c[8];
-      uint8_t b[8];
+  } else if constexpr (WALK == DQ_FLAT) {
+    const unsigned long long n = (unsigned long long)T * D, i0 = (unsigned long long)blockIdx.x * 2048 + threadIdx.x;
+    int t[8], c[8];
+    uint8_t b[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const unsigned long long i = i0 + 256 * j < n ? i0 + 256 * j : n - 1;   // past the end: not used
-        t[j] = (int)(i >> 32 ? i / (unsigned)D : (unsigned)i / (unsigned)D);
-        c[j] = (int)(i - (unsigned long long)t[j] * D);
-        b[j] = q[(size_t)t[j] * ldq + c[j]];
-      }
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (i0 + 256 * j < n)
-          y[(size_t)t[j] * ldy + c[j]] =
-              __float2bfloat16(code_value<FMT>(b[j]) * dequant_scale<FMT>(scale, sf, t[j], c[j], D / 128));
-      return;
+    for (int j = 0; j < 8; ++j) {
+      const unsigned long long i = i0 + 256 * j < n ? i0 + 256 * j : n - 1;   // past the end: not used
+      t[j] = (int)(i >> 32 ? i / (unsigned)D : (unsigned)i / (unsigned)D);
+      c[j] = (int)(i - (unsigned long long)t[j] * D);
+      b[j] = q[(size_t)t[j] * ldq + c[j]];
     }
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (i0 + 256 * j < n)
+        y[(size_t)t[j] * ldy + c[j]] =
+            __float2bfloat16(code_value<FMT>(b[j]) * dequant_scale<FMT>(scale, sf, t[j], c[j], D / 128));
+  } else {
     const int t = (int)(blockIdx.x / per_row), c0 = (int)(blockIdx.x % per_row) * 2048 + (int)threadIdx.x;
     const uint8_t* src = q + (size_t)t * ldq;
     uint8_t b[8];
@@ -742,19 +742,19 @@ static cudaError_t launch_dequant(const uint8_t* q, size_t ldq, const float* sca
   const bool vec = D % 16 == 0 && ldq % 16 == 0 && ldy % 8 == 0 && reinterpret_cast<uintptr_t>(q) % 16 == 0 &&
                    reinterpret_cast<uintptr_t>(y) % 16 == 0;
   // A block for 2048 columns of a row, or for 2048 elements of many narrow rows, where a
-  // division each costs less than idle threads (9135 x 37: 12.7 us and 4.0; x 401: 13.6
-  // and 10.4; x 1001: 19.5 and 24.1; 300 x 37: 1.6 and 3.1)
+  // division each costs less than idle threads (4095 x 37 by rows 5.8 us, 4096 x 37 flat
+  // 3.4; x 401: 6.1 and 5.4; x 509: 6.2 and 6.1)
   const bool flat = D <= 512 && T >= 4096;
   const unsigned per_row = vec ? (unsigned)(D / 16) : flat ? 0u : (unsigned)((D + 2047) / 2048);
   const unsigned long long blocks = vec    ? ((unsigned long long)T * per_row + 255) / 256
                                     : flat ? ((unsigned long long)T * D + 2047) / 2048
                                            : (unsigned long long)T * per_row;
   if (blocks >= (1ull << 31)) return cudaErrorInvalidValue;
-  if (vec)
-    launch_pdl(dequant_kernel<FMT, true>, (unsigned)blocks, 256, 0, st, q, ldq, scale, sf, T, D, y, ldy, per_row);
-  else
-    launch_pdl(dequant_kernel<FMT, false>, (unsigned)blocks, 256, 0, st, q, ldq, scale, sf, T, D, y, ldy, per_row);
-  return cudaGetLastError();
+  auto go = [&](auto kernel) {
+    return launch_pdl(kernel, (unsigned)blocks, 256, 0, st, q, ldq, scale, sf, T, D, y, ldy, per_row);
+  };
+  if (vec) return go(dequant_kernel<FMT, DQ_VEC>);
+  return flat ? go(dequant_kernel<FMT, DQ_FLAT>) : go(dequant_kernel<FMT, DQ_ROW>);
 }
 
 cudaError_t dequant_rows(const uint8_t* q, size_t ldq, const float* scale, const uint8_t* sf, int T, int D, int fmt,
