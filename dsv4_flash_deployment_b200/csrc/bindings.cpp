@@ -1002,7 +1002,7 @@ void dequant_rows(const Tensor& q, const Tensor& scale, int64_t fmt, const Tenso
   } else {
     check_vec(scale, "scale", q.size(0), at::kFloat, q);
   }
-  TORCH_CHECK(T < (1ll << 31) && D < (1ll << 31), "too large");
+  TORCH_CHECK(T < (1ll << 31) - 65536 && D < (1ll << 31) - 65536, "too large");
   const c10::cuda::CUDAGuard guard(q.device());
   CUDA_OK(dsv4::dequant_rows(reinterpret_cast<const uint8_t*>(q.data_ptr()), (size_t)q.stride(0),
                              mx ? nullptr : scale.data_ptr<float>(), mx ? scale.data_ptr<uint8_t>() : nullptr, (int)T,
@@ -1025,7 +1025,7 @@ void gemm_i8(const Tensor& x, const Tensor& xs, const Tensor& w, const Tensor& w
   const int64_t T = x.size(0), K = x.size(1), N = w.size(0);
   TORCH_CHECK(x.scalar_type() == at::kChar && w.scalar_type() == at::kChar, "x and w: int8");
   TORCH_CHECK(K >= 1 && K <= dsv4::kGemmI8MaxK, "K must be in 1..", str(dsv4::kGemmI8MaxK));
-  TORCH_CHECK(T < (1ll << 31) && N < (1ll << 31) - 128, "too many rows");
+  TORCH_CHECK(T < (1ll << 31) - 1024 && N < (1ll << 31) - 1024, "too many rows");
   check_rows(x, "x", T, K, x);
   check_rows(w, "w", N, K, x);
   check_vec(xs, "x scale", T, at::kFloat, x);

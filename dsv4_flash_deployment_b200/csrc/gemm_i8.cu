@@ -107,6 +107,14 @@ struct I8Smem {
   static_assert(kStages * kStage >= 128 * BN * 4, "a parked partial tile takes the stages' place");
 };
 
+// After an abort: waits, with mbar_wait's limit, for the copies into the stages last
+// asked for, which nobody took.
+template <int S>
+DSV4_DEV void drain_copies(uint64_t* full, int issued, uint32_t* err, uint32_t detail) {
+  for (int i = issued > S ? issued - S : 0; i < issued; ++i)
+    if (!mbar_wait(&full[i % S], (uint32_t)(i / S) & 1, nullptr, err, KID_GEMM, detail)) return;
+}
+
 // Range of k tiles of one split.
 DSV4_DEV int split_begin(int k_tiles, int splits, int i) { return (int)((long long)k_tiles * i / splits); }
 
@@ -159,7 +167,7 @@ __global__ void __launch_bounds__(kI8Threads, 1)
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  int csyncs = 0;
+  int csyncs = 0, issued = 0;   // issued: k tiles the producer has asked for
   if (threadIdx.x == 0) {
     for (int s = 0; s < S; ++s) {
       mbar_init(&full[s], 1);
@@ -204,6 +212,7 @@ __global__ void __launch_bounds__(kI8Threads, 1)
           mbar_arrive_expect_tx(&full[stage], L::kStage);
           tma_load_2d(sA + stage * L::kA, &map_w, &full[stage], kt * 128, m0);
           tma_load_2d(sB + stage * L::kB, &map_x, &full[stage], kt * 128, n0);
+          ++issued;
           if (++stage == S) stage = 0, phase ^= 1;
         }
       }
@@ -302,6 +311,7 @@ done:
     for (; csyncs < 2; ++csyncs) cluster_sync_all();
   tc_fence_before();
   __syncthreads();
+  if (warp == 0 && lane == 0 && *abort_flag) drain_copies<S>(full, issued, p.err, 16);
   if (warp == 1) {
     if (*abort_flag) {   // no tensor-core op may still use the TMEM
       if (lane == 0) umma_commit(drain);
@@ -454,6 +464,7 @@ __global__ void __launch_bounds__(kI8Threads, 1)
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = (int)cluster_ctarank();
+  int issued = 0;   // k tiles this CTA's producer has asked for
   const int pair = blockIdx.x >> 1, n_pairs = gridDim.x >> 1;
   if (threadIdx.x == 0) {
     for (int s = 0; s < S; ++s) {
@@ -501,6 +512,7 @@ __global__ void __launch_bounds__(kI8Threads, 1)
           if (rank == 0) mbar_arrive_expect_tx(&full[stage], bytes);
           tma_load_2d_pair(sA + stage * kPairA, &map_w, full0 + 8 * stage, kt * 128, m0);
           tma_load_2d_pair(sB + stage * kPairB, mx, full0 + 8 * stage, kt * 128, n0);
+          ++issued;
           if (++stage == S) stage = 0, phase ^= 1;
         }
       }
@@ -574,6 +586,9 @@ __global__ void __launch_bounds__(kI8Threads, 1)
   }
 done:
   __syncwarp();
+  __syncthreads();   // every warp has finished or given up
+  // the leader's barriers count both CTAs' copies; the other CTA waits for it below
+  if (*abort_flag && warp == 0 && rank == 0 && lane == 0) drain_copies<S>(full, issued, p.err, 26);
   if (*abort_flag && warp == 1 && rank == 0) {   // no product may still use either CTA's TMEM
     if (lane == 0)
       asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(drain))

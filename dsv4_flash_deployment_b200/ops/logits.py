@@ -95,10 +95,10 @@ class RowRules:
 
 def apply_logits_rules(logits: torch.Tensor, rules: RowRules, history: TokenHistory | None = None,
                        out: torch.Tensor | None = None) -> torch.Tensor:
-    """Applies ``rules`` to ``logits`` [S, V] (bf16, fp16 or fp32, contiguous rows) into
-    ``out`` (None: in place; else it may not overlap the logits) and returns it.
-    ``history`` is needed with penalties.  A slot or mask row outside its table leaves
-    the row without that rule and is reported in the device error word."""
+    """Applies ``rules`` to ``logits`` [S, V] (bf16, fp16 or fp32, contiguous rows, up to
+    65535 of them) into ``out`` (None: in place; else it may not overlap the logits) and
+    returns it.  ``history`` is needed with penalties.  A slot or mask row outside its
+    table leaves the row without that rule and is reported in the device error word."""
     r = rules
     if r.slots is not None and history is None:
         raise ValueError("penalties need a token history")
