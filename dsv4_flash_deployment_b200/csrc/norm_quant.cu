@@ -422,8 +422,8 @@ __global__ void __launch_bounds__(MAXT, MINB) norm_quant_kernel(NormQuantParams 
 // Every other row: any alignment, any width up to 32768.  A block per row, which waits in
 // shared memory (as s w in fp32; MX8: as s) between the two halves; off 16-byte
 // boundaries element accesses, neighbours in a warp, eight in flight a thread (777 x 5003
-// fp32: 9.8 us, with four 11.0; in 16-byte pieces from the boundary before the row 13.2,
-// since a lane's columns then lie apart in the weights and in shared memory).  WARP: a
+// fp32: 9.8 us then, with four 11.0; in 16-byte pieces from the boundary before the row
+// 13.2, since a lane's columns then lie apart in the weights and in shared memory).  WARP: a
 // warp per row, 8 rows a block.
 constexpr int kStagedWarps = 8;
 template <typename TX, typename TW, int FMT, bool ALIGNED, bool WARP>
@@ -645,12 +645,18 @@ __global__ void __launch_bounds__(256) dequant_kernel(const uint8_t* q, size_t l
 template <typename TX, typename TW, int FMT>
 static cudaError_t launch_norm(const NormQuantParams& p, bool vec, int sms, cudaStream_t st) {
   if (!vec || p.D > 2 * 8 * kNormThreads) {
-    // 8 columns a thread while the rows leave SMs idle, 16 once they come in waves
-    const int each = p.T <= 2 * sms ? 8 : 16;
-    const int nt = std::min(kNormThreads, std::max(32, (p.D / each + 31) / 32 * 32));
+    // 8 to 32 columns a thread, as many as it takes for the rows to be resident together (1024
+    // threads an SM), and 256 threads, four blocks an SM, rather than two of up to 384 (fp32
+    // 777 x 5003 9.9 us with 16, 8.4 so; 9598 x 6177 166 and 144; 4096 x 8200 59 and 48; bf16
+    // 2000 x 12001 54.6 and 49.0; 777 x 1001 5.2 and 4.2).
+    auto warps = [](int n) { return std::max(32, (n + 31) / 32 * 32); };
+    const int fit = 1024 / std::min(32, (p.T + sms - 1) / sms) / 32 * 32;
+    int nt = std::max(warps(p.D / 32), std::min(warps(p.D / 8), fit));
+    if (p.T > 4 * sms && nt > 256 && nt <= 384) nt = 256;
+    nt = std::min(kNormThreads, nt);
     const size_t row_bytes = (size_t)(p.D + 3) / 4 * 16;
     // very many narrow rows: a warp each (9135 x 37 fp16: 9.9 us with a block a row, 5.2 so;
-    // x 1001 bf16: 21.8 and 20.4; 1200 x 1001: 6.2 and 6.6)
+    // 1200 x 1001 bf16: 5.4 and 6.6)
     if (!vec && p.D <= 1024 && p.T >= 16 * sms)
       return launch_pdl(norm_quant_staged_kernel<TX, TW, FMT, false, true>, (unsigned)((p.T + kStagedWarps - 1) / kStagedWarps),
                         32 * kStagedWarps, kStagedWarps * row_bytes, st, p);
