@@ -14,9 +14,10 @@
 // between the two halves.
 //
 // Rows that hold an infinity or NaN come out as NaN: NaN scale, codes 0 (MX8:
-// scale byte 0xFF, which the tensor core reads as NaN).  Finite rows whose squares
-// pass fp32's range are scaled by 2^-96 and summed again (the eps is lost there:
-// it is under 2^-60 of the mean).
+// scale byte 0xFF, which the tensor core reads as NaN), and so do rows whose y passes
+// fp32's range.  A row where only a partial result passes it is worked out again
+// (far_row): squares are those of s scaled by 2^-96 (the eps is lost there: it is under
+// 2^-60 of the mean), and where s w passes the range the root comes first, y = (s r) w.
 #include "common.cuh"
 #include "kernels.h"
 
@@ -250,13 +251,25 @@ DSV4_DEV F2 norm_once(F2 s, F2 w, Root r) {
 DSV4_DEV bool between_codes(F2 y) {
   return (__float_as_uint(y.x) & 0x7ffffu) == 0 || (__float_as_uint(y.y) & 0x7ffffu) == 0;
 }
+// a b + c to odd; c is small beside a b
+DSV4_DEV float fma_odd(float a, float b, float c) {
+  const float y0 = a * b, e0 = fmaf(a, b, -y0);      // a b = y0 + e0
+  c += e0;
+  const float y = y0 + c, rest = c - (y - y0);
+  uint32_t bits = __float_as_uint(y);
+  if (rest != 0.f && !(bits & 1u)) bits += (__float_as_uint(rest) ^ bits) >> 31 ? 0xffffffffu : 1u;
+  return __uint_as_float(bits);
+}
 DSV4_DEV float norm_odd(float s, float w, Root r) {
   const float v = s * w, ev = fmaf(s, w, -v);
-  const float y0 = v * r.hi, e0 = fmaf(v, r.hi, -y0);      // v r.hi = y0 + e0
-  const float c = fmaf(ev, r.hi, v * r.lo) + e0, y = y0 + c, rest = c - (y - y0);
-  uint32_t b = __float_as_uint(y);
-  if (rest != 0.f && !(b & 1u)) b += (__float_as_uint(rest) ^ b) >> 31 ? 0xffffffffu : 1u;
-  return __uint_as_float(b);
+  return fma_odd(v, r.hi, fmaf(ev, r.hi, v * r.lo));
+}
+// y of a row that passes the range on the way: where s w does, the root comes first
+template <int FMT>
+DSV4_DEV float norm_far(float s, float w, Root r) {
+  if (fabsf(s * w) < INFINITY) return FMT == Q8_MX8 ? norm_odd(s, w, r) : s * w * r.hi;
+  const float v = s * r.hi;
+  return FMT == Q8_MX8 ? fma_odd(v, w, fmaf(s, r.lo, fmaf(s, r.hi, -v)) * w) : v * w;
 }
 
 }  // namespace
@@ -266,6 +279,75 @@ constexpr float kDown = 1.2621774483536189e-29f;   // 2^-96
 DSV4_DEV uint32_t mx_exp(float amax, bool bad) { return bad ? 255u : pow2_ceil_exp(fmaxf(amax, 1e-4f), 1.f / 448.f); }
 // 1 / 2^(e - 127), exact: e is under 248 for finite rows
 DSV4_DEV float mx_inv(uint32_t e, bool bad) { return bad ? 0.f : exp_to_f32(254 - e); }
+
+// A row (with weights) whose sum of squares ss or whose y by way of s w is not finite, by
+// all its threads: from memory again, an element at a time, since such rows are rare.
+// Three passes: the sum of the squares scaled down, the largest y, the codes.
+template <typename TX, typename TW, int FMT, bool WARP, int MAXT, typename Sum>
+DSV4_DEV void far_row(const NormQuantParams& p, int t, int tid, int nt, Sum ss, RowRed<Sum>& red) {
+  constexpr bool kMx = FMT == Q8_MX8;
+  constexpr float top = FMT == Q8_I8 ? 127.f : 448.f;
+  const TX* ro = p.res_out ? static_cast<const TX*>(p.res_out) + (size_t)t * p.ldro : nullptr;
+  const TW* w = static_cast<const TW*>(p.w);
+  const int D = p.D;
+  // also: the row's residual_out is written, and `red` has been read
+  auto sync = [] {
+    if constexpr (WARP)
+      __syncwarp();
+    else
+      __syncthreads();
+  };
+  sync();
+  // residual_out may be the residual itself and then holds the rounded sum: the ratio of
+  // two such rows differs by that rounding only
+  float mx = 0.f, down = 1.f;
+  Root r;
+  if ((float)ss < INFINITY) {
+    r = inv_root(ss, p, p.eps);
+  } else {
+    down = kDown;
+    ss = 0;
+#pragma unroll 1
+    for (int c = tid; c < D; c += nt) {
+      const float s = row_again<TX>(p, ro, t, c) * kDown;
+      ss += (Sum)s * (Sum)s;
+    }
+    row_sum_max<WARP, MAXT>(ss, mx, red);
+    sync();
+    r = inv_root(ss, p, 0.f);
+  }
+  auto y_at = [&](int c) { return norm_far<FMT>(row_again<TX>(p, ro, t, c) * down, to_f(w[c]), r); };
+  mx = 0.f;
+#pragma unroll 1
+  for (int c = tid; c < D; c += nt) mx = max_nan(mx, fabsf(y_at(c)));
+  Sum unused = ss;
+  row_sum_max<WARP, MAXT>(unused, mx, red);
+  const bool bad = !((float)ss < INFINITY) || !(mx < INFINITY);
+  float k8 = 0.f, up = 1.f;
+  if constexpr (!kMx) {
+    if (tid == 0) p.scale[t] = bad ? __uint_as_float(0x7fffffffu) : fmaxf(mx, 1e-30f) / top;
+    k8 = code_scale(1.f, mx, top, &up);
+  }
+  uint8_t* q = p.q + (size_t)t * p.ldq;
+#pragma unroll 1
+  for (int c = 4 * tid; c < D; c += 4 * nt) {   // MX8: D % 128 == 0, so a warp's lanes stay together
+    float y[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) y[j] = c + j < D ? y_at(c + j) : 0.f;
+    if constexpr (kMx) {                        // 8 lanes hold a block of 32 columns
+      float am = fmaxf(fmaxf(fabsf(y[0]), fabsf(y[1])), fmaxf(fabsf(y[2]), fabsf(y[3])));
+#pragma unroll
+      for (int o = 1; o < 8; o <<= 1) am = fmaxf(am, __shfl_xor_sync(0xffffffffu, am, o));
+      const uint32_t e = mx_exp(am, bad);
+      k8 = mx_inv(e, bad);
+      if ((tid & 7) == 0) p.sf[sf_chunk_offset(t, c >> 5, D / 128)] = (uint8_t)e;
+    }
+    const uint32_t pk = bad ? 0u : codes4<FMT>({y[0] * up, y[1] * up}, {y[2] * up, y[3] * up}, k8);
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (c + j < D) q[c + j] = (uint8_t)(pk >> (8 * j));
+  }
+}
 
 // Rows of up to 8192 columns, all on 16-byte boundaries, 8 columns to a group.
 //
@@ -348,33 +430,16 @@ __global__ void __launch_bounds__(MAXT, MINB) norm_quant_kernel(NormQuantParams 
     }
     Sum ss = kMx ? Sum(dx + dy) : Sum(sq.x + sq.y);
     row_sum_max<WARP, MAXT>(ss, mx, red[turn]);
-    bool bad;
+    bool bad = false;
     Root r{1.f, 0.f};
     if (!has_w) {
       bad = ss != ss || !(mx < INFINITY);   // no norm: squares may overflow, infinities and NaN may not pass
-    } else if ((float)ss < INFINITY && mx < INFINITY) {
-      bad = false;
+    } else {
       r = inv_root(ss, p, p.eps);
-    } else {   // all threads of the row alike: the row again, scaled by 2^-96
-      ss = 0;
-      mx = 0.f;
-#pragma unroll
-      for (int k = 0; k < PER; ++k)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const int c = col(k) + j;
-          // residual_out may be the residual itself and then holds the rounded sum: the
-          // ratio of two such rows differs by that rounding only
-          float s = c < D ? row_again<TX>(p, ro, t, c) * kDown : 0.f;
-          ss += (Sum)s * (Sum)s;
-          if (c < D && !kMx) s *= to_f(static_cast<const TW*>(p.w)[c]);
-          mx = max_nan(mx, fabsf(s));
-          (j & 1 ? v[k][j >> 1].y : v[k][j >> 1].x) = s;
-        }
-      if constexpr (!WARP) __syncthreads();   // red is still being read
-      row_sum_max<WARP, MAXT>(ss, mx, red[turn]);
-      bad = !((float)ss < INFINITY) || !(mx < INFINITY);
-      if (!bad) r = inv_root(ss, p, 0.f);
+      if (!((float)ss < INFINITY) || !(r.hi * mx < INFINITY)) {   // all threads of the row alike
+        far_row<TX, TW, FMT, WARP, MAXT>(p, t, tid, nt, ss, red[turn]);
+        continue;
+      }
     }
     uint8_t* q = p.q + (size_t)t * p.ldq;
     constexpr float top = FMT == Q8_I8 ? 127.f : 448.f;
@@ -432,7 +497,7 @@ __global__ void __launch_bounds__(kNormThreads, 2) norm_quant_staged_kernel(Norm
   extern __shared__ __align__(16) float s_rows[];   // a row: D, rounded up to 4
   constexpr bool kMx = FMT == Q8_MX8;
   using Sum = typename std::conditional<kMx, double, float>::type;
-  __shared__ RowRed<Sum> red[2];
+  __shared__ RowRed<Sum> red;
   const int tid = WARP ? threadIdx.x & 31 : threadIdx.x, nt = WARP ? 32 : blockDim.x, D = p.D;
   const int t = WARP ? (int)blockIdx.x * kStagedWarps + (int)(threadIdx.x >> 5) : (int)blockIdx.x;
   if (WARP && t >= p.T) return;   // a warp alike; no barrier of the block follows
@@ -515,26 +580,17 @@ __global__ void __launch_bounds__(kNormThreads, 2) norm_quant_staged_kernel(Norm
     }
   }
   if (tid < (4 - D % 4) % 4) s_row[D + tid] = 0.f;
-  row_sum_max<WARP, kNormThreads>(ss, mx, red[0]);
-  bool bad;
+  row_sum_max<WARP, kNormThreads>(ss, mx, red);
+  bool bad = false;
   Root r{1.f, 0.f};
   if (!w) {
     bad = ss != ss || !(mx < INFINITY);
-  } else if ((float)ss < INFINITY && mx < INFINITY) {
-    bad = false;
-    r = inv_root(ss, p, p.eps);
   } else {
-    ss = 0;
-    mx = 0.f;
-    for (int c = tid; c < D; c += nt) {
-      const float s = row_again<TX>(p, ro, t, c) * kDown;
-      ss += (Sum)s * (Sum)s;
-      s_row[c] = kMx ? s : s * to_f(w[c]);
-      mx = max_nan(mx, fabsf(s_row[c]));
+    r = inv_root(ss, p, p.eps);
+    if (!((float)ss < INFINITY) || !(r.hi * mx < INFINITY)) {
+      far_row<TX, TW, FMT, WARP, kNormThreads>(p, t, tid, nt, ss, red);
+      return;
     }
-    row_sum_max<WARP, kNormThreads>(ss, mx, red[1]);
-    bad = !((float)ss < INFINITY) || !(mx < INFINITY);
-    if (!bad) r = inv_root(ss, p, 0.f);
   }
   if constexpr (WARP)   // the row is complete
     __syncwarp();
