@@ -368,7 +368,7 @@ __global__ void __launch_bounds__(MAXT, MINB) norm_quant_kernel(NormQuantParams 
   const int rows = WARP ? (int)gridDim.x * 4 : (int)gridDim.x;
   const int D = p.D;
   const bool has_res = p.res != nullptr, has_w = p.w != nullptr;
-  constexpr bool kMx = FMT == Q8_MX8;   // keeps s in registers (no row maximum is needed), the others s w
+  constexpr bool kMx = FMT == Q8_MX8;   // keeps s in registers, the others s w
   using Sum = typename std::conditional<kMx, double, float>::type;
   __shared__ RowRed<Sum> red[2];
   auto col = [&](int k) { return 8 * (tid + k * nt); };
@@ -425,8 +425,15 @@ __global__ void __launch_bounds__(MAXT, MINB) norm_quant_kernel(NormQuantParams 
 #pragma unroll
         for (int j = 0; j < 4; ++j) v[k][j] = mul2(v[k][j], f[j]);
       }
+      if (kMx && has_w && col(k) < D) {   // only to see whether every s w is finite
+        F2 f[4];
+        floats_of(wv[k], f);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) mx = abs_max(mx, v[k][j]);
+        for (int j = 0; j < 4; ++j) mx = abs_max(mx, mul2(v[k][j], f[j]));
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) mx = abs_max(mx, v[k][j]);
+      }
     }
     Sum ss = kMx ? Sum(dx + dy) : Sum(sq.x + sq.y);
     row_sum_max<WARP, MAXT>(ss, mx, red[turn]);
@@ -517,7 +524,7 @@ __global__ void __launch_bounds__(kNormThreads, 2) norm_quant_staged_kernel(Norm
         const int c = 8 * min(g0 + i * nt, D / 8 - 1);   // past the end: not used
         a[i] = ld_vec8(x + c);
         if (res) b[i] = ld_vec8(res + c);
-        if (w && !kMx) wc[i] = ld_vec8(w + c);
+        if (w) wc[i] = ld_vec8(w + c);
       }
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
@@ -547,8 +554,14 @@ __global__ void __launch_bounds__(kNormThreads, 2) norm_quant_staged_kernel(Norm
 #pragma unroll
           for (int j = 0; j < 4; ++j) v[j] = mul2(v[j], f[j]);
         }
+        if (w && kMx) {
+          floats_of(wc[i], f);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) mx = abs_max(mx, v[j]);
+          for (int j = 0; j < 4; ++j) mx = abs_max(mx, mul2(v[j], f[j]));
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) mx = abs_max(mx, v[j]);
+        }
         *reinterpret_cast<float4*>(s_row + c) = make_float4(v[0].x, v[0].y, v[1].x, v[1].y);
         *reinterpret_cast<float4*>(s_row + c + 4) = make_float4(v[2].x, v[2].y, v[3].x, v[3].y);
       }
@@ -563,7 +576,7 @@ __global__ void __launch_bounds__(kNormThreads, 2) norm_quant_staged_kernel(Norm
         const int c = min(c0 + i * nt, D - 1);   // past the end: not used
         a[i] = x[c];
         if (res) b[i] = res[c];
-        if (w && !kMx) wc[i] = w[c];
+        if (w) wc[i] = w[c];
       }
 #pragma unroll
       for (int i = 0; i < U; ++i) {
@@ -573,9 +586,9 @@ __global__ void __launch_bounds__(kNormThreads, 2) norm_quant_staged_kernel(Norm
         if (res) s += to_f(b[i]);
         if (ro) ro[c] = from_f<TX>(s);
         ss += (Sum)s * (Sum)s;
-        const float sw = w && !kMx ? s * to_f(wc[i]) : s;
+        const float sw = w ? s * to_f(wc[i]) : s;
         mx = max_nan(mx, fabsf(sw));
-        s_row[c] = sw;
+        s_row[c] = kMx ? s : sw;
       }
     }
   }

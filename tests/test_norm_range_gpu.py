@@ -49,7 +49,7 @@ def _check(got, x, w, eps, fmt, res=None):
     return fine
 
 
-@pytest.mark.parametrize("fmt", ["i8", "e4m3"])
+@pytest.mark.parametrize("fmt", ["i8", "e4m3", "mx8"])
 @pytest.mark.parametrize("t,d,off", SHAPES)
 @pytest.mark.parametrize("dt", [F32, BF])
 @pytest.mark.parametrize("eps", [1e-6, 4.0])
@@ -72,7 +72,7 @@ def test_products_past_the_range(t, d, off, dt, eps, fmt):
     assert fine[:6].tolist() == [True, True, True, False, True, True]
 
 
-@pytest.mark.parametrize("fmt", ["i8", "e4m3"])
+@pytest.mark.parametrize("fmt", ["i8", "e4m3", "mx8"])
 @pytest.mark.parametrize("t,d,off", SHAPES)
 @pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
 def test_weights_that_are_not_finite(t, d, off, bad, fmt):
