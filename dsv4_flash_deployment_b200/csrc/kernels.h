@@ -397,6 +397,7 @@ struct NormQuantParams {
   const void* w;         // [D], or null: no norm, only the quantization of x (+ res)
   float eps;
   double inv_d;          // 1 / D (set by norm_quant)
+  bool in_place;         // res_out is x or res (set by norm_quant)
   uint8_t* q;            // [T, D] codes, rows ldq apart
   size_t ldq;
   float* scale;          // [T] (I8, E4M3)

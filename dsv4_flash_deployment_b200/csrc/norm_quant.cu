@@ -133,10 +133,11 @@ DSV4_DEV void st_vec8(T* p, const F2 (&x)[4]) {
   }
 }
 
-// x + residual of one column, as it can still be read after residual_out was written
+// x + residual of one column after residual_out was written: its rounded value where that
+// took the place of an input
 template <typename TX>
-DSV4_DEV float row_again(const NormQuantParams& p, const TX* ro, int t, int c) {
-  if (ro) return to_f(ro[c]);
+DSV4_DEV float row_again(const NormQuantParams& p, int t, int c) {
+  if (p.in_place) return to_f(static_cast<const TX*>(p.res_out)[(size_t)t * p.ldro + c]);
   const float a = to_f(static_cast<const TX*>(p.x)[(size_t)t * p.ldx + c]);
   return p.res ? a + to_f(static_cast<const TX*>(p.res)[(size_t)t * p.ldr + c]) : a;
 }
@@ -287,7 +288,6 @@ template <typename TX, typename TW, int FMT, bool WARP, int MAXT, typename Sum>
 DSV4_DEV void far_row(const NormQuantParams& p, int t, int tid, int nt, Sum ss, RowRed<Sum>& red) {
   constexpr bool kMx = FMT == Q8_MX8;
   constexpr float top = FMT == Q8_I8 ? 127.f : 448.f;
-  const TX* ro = p.res_out ? static_cast<const TX*>(p.res_out) + (size_t)t * p.ldro : nullptr;
   const TW* w = static_cast<const TW*>(p.w);
   const int D = p.D;
   // also: the row's residual_out is written, and `red` has been read
@@ -298,8 +298,6 @@ DSV4_DEV void far_row(const NormQuantParams& p, int t, int tid, int nt, Sum ss, 
       __syncthreads();
   };
   sync();
-  // residual_out may be the residual itself and then holds the rounded sum: the ratio of
-  // two such rows differs by that rounding only
   float mx = 0.f, down = 1.f;
   Root r;
   if ((float)ss < INFINITY) {
@@ -309,14 +307,14 @@ DSV4_DEV void far_row(const NormQuantParams& p, int t, int tid, int nt, Sum ss, 
     ss = 0;
 #pragma unroll 1
     for (int c = tid; c < D; c += nt) {
-      const float s = row_again<TX>(p, ro, t, c) * kDown;
+      const float s = row_again<TX>(p, t, c) * kDown;
       ss += (Sum)s * (Sum)s;
     }
     row_sum_max<WARP, MAXT>(ss, mx, red);
     sync();
     r = inv_root(ss, p, 0.f);
   }
-  auto y_at = [&](int c) { return norm_far<FMT>(row_again<TX>(p, ro, t, c) * down, to_f(w[c]), r); };
+  auto y_at = [&](int c) { return norm_far<FMT>(row_again<TX>(p, t, c) * down, to_f(w[c]), r); };
   mx = 0.f;
 #pragma unroll 1
   for (int c = tid; c < D; c += nt) mx = max_nan(mx, fabsf(y_at(c)));
@@ -797,6 +795,7 @@ cudaError_t norm_quant(NormQuantParams p, int xtype, int wtype, int fmt, int sms
   static_assert(4 * kNormMaxD <= 200 * 1024, "the widest row fits shared memory");
   if (p.D > kNormMaxD) return cudaErrorInvalidValue;
   p.inv_d = 1.0 / p.D;
+  p.in_place = p.res_out && (p.res_out == p.x || p.res_out == p.res);
   const size_t ex = xtype == F_F32 ? 4 : 2, ew = wtype == F_F32 ? 4 : 2;
   auto al = [](const void* q, size_t ld_bytes) {
     return q == nullptr || (reinterpret_cast<uintptr_t>(q) % 16 == 0 && ld_bytes % 16 == 0);

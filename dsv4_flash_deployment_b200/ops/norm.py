@@ -43,10 +43,11 @@ def rms_norm_quant(x: torch.Tensor, weight: torch.Tensor, eps: float, fmt: str =
     x's type or fp32; ``eps`` at least 1e-30.  Returns ``(q, scale)``, or with a
     residual ``(q, scale, residual_out)`` with the sum rounded to x's type
     (``residual_out`` may be ``residual`` or ``x`` itself; the norm takes the sum
-    before its rounding).  ``q_out`` / ``scale_out``: buffers to write
-    (:func:`empty_rows`); apart from ``residual_out`` being an input whole, no output
-    may overlap an input.  Rows that hold an infinity or NaN come out as NaN (their
-    scale is NaN)."""
+    before its rounding, except that a row whose squares or products with the weight
+    pass fp32's range takes the rounded sum where it replaced an input).  ``q_out`` /
+    ``scale_out``: buffers to write (:func:`empty_rows`); apart from ``residual_out``
+    being an input whole, no output may overlap an input.  Rows that hold an infinity
+    or NaN, or whose y passes fp32's range, come out as NaN (their scale is NaN)."""
     f = Q8_FMT.get(fmt)
     if f is None:
         raise ValueError(f"fmt {fmt!r}: one of {sorted(Q8_FMT)}")

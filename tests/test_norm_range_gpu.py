@@ -91,3 +91,22 @@ def test_weights_that_are_not_finite(t, d, off, bad, fmt):
     got = Q.rms_norm_quant(x, w, 1e-6, fmt)
     _done()
     assert _check(got, x, w, 1e-6, fmt).all()
+
+
+@pytest.mark.parametrize("fmt", ["i8", "e4m3", "mx8"])
+@pytest.mark.parametrize("t,d,off", SHAPES)
+def test_sum_before_its_rounding_past_the_range(t, d, off, fmt):
+    """The norm takes x + residual before residual_out's rounding also where the squares
+    overflow; residual_out in place of an input holds the rounded sum there, and the
+    codes are then those of the rounded sum (documented)."""
+    g = _gen(d + 2)
+    x, res = ((1e25 * torch.randn(t, d + 8, device="cuda", generator=g)).to(BF)[:, off:off + d] for _ in range(2))
+    w = torch.rand(d, device="cuda", generator=g) + 0.5
+    got = Q.rms_norm_quant(x, w, 1e-6, fmt, residual=res)
+    _done()
+    assert _check(got, x, w, 1e-6, fmt, res).all()
+    x1 = x.clone(memory_format=torch.contiguous_format)
+    again = Q.rms_norm_quant(x1, w, 1e-6, fmt, residual=res, residual_out=x1)
+    _done()
+    assert torch.equal(x1, got[2])
+    assert _check(again, x1, w, 1e-6, fmt).all()
