@@ -193,10 +193,13 @@ def row_quant(y: torch.Tensor, fmt: str) -> tuple[torch.Tensor, torch.Tensor]:
 
 def add_rms_norm(x: torch.Tensor, w: torch.Tensor, eps: float,
                  residual: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
-    """(RMSNorm of x + residual in fp32, not rounded; the sum in ``x.dtype``)."""
+    """(RMSNorm of x + residual in fp32, not rounded further; the sum in ``x.dtype``).
+    Squares and products are taken in 64 bits, since either may pass fp32's range where
+    the norm does not."""
     s = x.float() if residual is None else x.float() + residual.float()
-    y = s * torch.rsqrt(s.square().mean(-1, keepdim=True) + eps) * w.float()
-    return y, s.to(x.dtype)
+    d = s.double()
+    y = d * torch.rsqrt(d.square().mean(-1, keepdim=True) + eps) * w.double()
+    return y.float(), s.to(x.dtype)
 
 
 def i8_linear(xq: torch.Tensor, xs: torch.Tensor, wq: torch.Tensor, ws: torch.Tensor,
