@@ -8,7 +8,7 @@ model step, so all ranks step in lockstep.  Per step:
   all      apply the adds/cancels to the local scheduler; if any rank has
            work, run a real step (or a 1-token dummy step on a reserved slot
            when this rank has none, to join the step's collectives)
-  all      gather     [(request id, token, finished, reason, logprob)] -> rank 0
+  all      gather     [(request id, token, finished, reason, logprob[, error])] -> rank 0
 
 The messages travel on a control channel (engine/control.py): by default a
 shared-memory file for the ranks of one node (tens of microseconds per round
@@ -36,6 +36,7 @@ from dataclasses import dataclass, field
 
 from ..models.model import SeqChunk, StepMeta
 from .control import GlooControl
+from .engine import outputs
 
 
 @dataclass
@@ -52,6 +53,7 @@ class GlobalRequest:
     t_first_token: float | None = None
     t_done: float | None = None
     logprobs: list = field(default_factory=list)   # per token when the request asked for them
+    error: str | None = None      # why its rank's engine ended it
 
 
 class _SchedView:
@@ -89,6 +91,11 @@ class _SchedView:
         return _S()
 
 
+def _error(req) -> tuple:
+    """What an event carries besides the rest when the request ended with an error."""
+    return () if req.error is None else (req.error,)
+
+
 def _local_step(engine, msg: dict, rank: int, id_map: dict, pad_slot: int, replicated: bool = False) -> list[tuple]:
     """Applies a control message to this rank's engine and runs its part of the step."""
     for gid, r, prompt, mt, ignore_eos, stop_ids, temperature, extra in msg["adds"]:
@@ -113,13 +120,13 @@ def _local_step(engine, msg: dict, rank: int, id_map: dict, pad_slot: int, repli
     for req, tok in events:
         gid = id_map.get(req.req_id)
         lp = req.logprobs[len(req.output) - 1] if tok is not None and req.logprobs else None
-        out.append((gid, tok, req.finished, req.finish_reason, lp))
+        out.append((gid, tok, req.finished, req.finish_reason, lp, *_error(req)))
     # requests finished without an event this step (cancelled before scheduling)
     for key in [k for k in id_map if isinstance(k, tuple)]:
         req = id_map[key]
         if req.finished:
             if not any(e[0] == key[1] for e in out):
-                out.append((key[1], None, True, req.finish_reason, None))
+                out.append((key[1], None, True, req.finish_reason, None, *_error(req)))
             del id_map[key]
             id_map.pop(req.req_id, None)
     if replicated and rank != 0:
@@ -189,7 +196,7 @@ class DistributedEngine:
         now = time.perf_counter()
         events = []
         for evs in gathered:
-            for gid, tok, fin, reason, lp in evs or []:
+            for gid, tok, fin, reason, lp, *error in evs or []:
                 g = self.live.get(gid)
                 if g is None:
                     continue
@@ -201,6 +208,7 @@ class DistributedEngine:
                         g.t_first_token = now
                 if fin:
                     g.finished, g.finish_reason, g.t_done = True, reason, now
+                    g.error = error[0] if error else None
                     if g.rank >= 0:
                         self.load[g.rank] -= 1
                     del self.live[gid]
@@ -223,7 +231,7 @@ class DistributedEngine:
         reqs = [self.add_request(p, max_new_tokens, ignore_eos, **sampling) for p in prompts]
         while not all(r.finished for r in reqs):
             self.step()
-        return [r.output for r in reqs]
+        return outputs(reqs)
 
 
 def worker_loop(local_engine, cpu_group=None, pad_slot: int | None = None, replicated: bool = False,

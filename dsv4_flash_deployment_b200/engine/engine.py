@@ -28,6 +28,14 @@ from ..ops.gemm import ErrorWord
 from .scheduler import Request, Scheduler
 
 
+def outputs(reqs) -> list[list[int]]:
+    """The finished requests' tokens; RuntimeError with the first error among them."""
+    for r in reqs:
+        if r.error is not None:
+            raise RuntimeError(r.error)
+    return [r.output for r in reqs]
+
+
 class Engine:
     """``bucket``: graph-replayed steps are padded to bucketed token / sampled-row
     counts (``StepMeta.padded``), so a serving run with changing batch
@@ -123,13 +131,14 @@ class Engine:
         return sp
 
     def step(self) -> list[tuple[Request, int | None]]:
-        chunks = self.sched.schedule()
+        chunks, masks, failed = self._masked(self.sched.schedule())
         if not chunks:
-            return []
+            return failed
         meta = StepMeta(self.cfg, [SeqChunk(c.req.slot, c.start_pos, c.tokens, c.sample,
                                             temperature=c.req.temperature, top_k=c.req.top_k, top_p=c.req.top_p,
-                                            logprobs=c.req.want_logprobs, seed=c.req.seed, **self._rules_of(c))
-                                   for c in chunks])
+                                            logprobs=c.req.want_logprobs, seed=c.req.seed, rules=c.req.rules,
+                                            n_prompt=len(c.req.prompt), mask=m)
+                                   for c, m in zip(chunks, masks)])
         ids = self.run_meta(meta)
         if meta.want_lp:
             it = iter(self.last_logprobs)
@@ -138,20 +147,25 @@ class Engine:
                     e = next(it)
                     if e is not None:
                         c.req.logprobs.append(e)
-        return self.sched.commit(chunks, ids)
+        return failed + self.sched.commit(chunks, ids)
 
-    def _rules_of(self, c) -> dict:
-        r = c.req.rules
-        if r is None:
-            return {}
-        mask = None
-        if c.sample:
-            try:
-                mask = r.words(c.req.output, self.cfg.vocab_size, self.eos_id)
-            except Exception as e:  # noqa: BLE001  (a request's own grammar object: only that request ends)
-                c.req.error = f"grammar: {type(e).__name__}: {e}"
-                self.sched.cancel(c.req)
-        return {"rules": r, "n_prompt": len(c.req.prompt), "mask": mask}
+    def _masked(self, chunks) -> tuple[list, list, list]:
+        """The chunks to run and the grammar mask of each (None: any token).  A request
+        whose grammar fails ends here, with its error and without a token; its event is
+        in the third list."""
+        run, masks, failed = [], [], []
+        for c in chunks:
+            mask = None
+            if c.sample and c.req.rules is not None:
+                try:
+                    mask = c.req.rules.words(c.req.output, self.cfg.vocab_size, self.eos_id)
+                except Exception as e:  # noqa: BLE001  (a request's own grammar object: only that request ends)
+                    self.sched.fail(c.req, f"grammar: {type(e).__name__}: {e}")
+                    failed.append((c.req, None))
+                    continue
+            run.append(c)
+            masks.append(mask)
+        return run, masks, failed
 
     last_logprobs: list = []   # per sampled row of the last step that asked for log-probabilities
 
@@ -233,11 +247,12 @@ class Engine:
     def generate(self, prompts: list[list[int]], max_new_tokens: int, ignore_eos: bool = False,
                  **sampling) -> list[list[int]]:
         """Runs the prompts to completion; ``sampling``: :meth:`add_request`'s decoding
-        options (temperature, top_k, top_p, seed, logprobs, penalties, biases, grammar)."""
+        options (temperature, top_k, top_p, seed, logprobs, penalties, biases, grammar).
+        RuntimeError when a request ended with an error (after the others have run)."""
         reqs = [self.add_request(p, max_new_tokens, ignore_eos, **sampling) for p in prompts]
         while not all(r.finished for r in reqs):
             self.step()
-        return [r.output for r in reqs]
+        return outputs(reqs)
 
     def check_errors(self) -> None:
         ErrorWord.check(self.model.dev)

@@ -44,7 +44,7 @@ class Request:
     want_logprobs: int | None = None  # alternatives per generated token (None: no log-probabilities)
     seed: int | None = None           # samples depend on (seed, position) only
     rules: object = None              # models.sampling.TokenRules: penalties, biases, grammar
-    error: str | None = None          # why the engine cancelled it (a grammar that failed)
+    error: str | None = None          # why the engine ended it (a grammar that failed)
     slot: int = -1
     n_prefilled: int = 0
     output: list[int] = field(default_factory=list)
@@ -130,6 +130,12 @@ class Scheduler:
 
     def cancel(self, req: Request) -> None:
         req.cancelled = True
+
+    def fail(self, req: Request, error: str) -> None:
+        """Ends a request at once, with the reason; its slot is free for the next step."""
+        req.cancelled = True
+        req.error = error
+        self._finish(req, "cancelled")
 
     def schedule(self) -> list[ScheduledChunk]:
         # drop cancelled requests

@@ -219,6 +219,11 @@ class EngineLoop:
             # finished (length / stop / cancelled) requests
             for rid in [rid for rid, s in self._live.items() if s.req.finished]:
                 s = self._live.pop(rid)
+                error = getattr(s.req, "error", None)
+                if error is not None:         # the engine ended this request (a grammar that failed)
+                    self.stats["failed"] += 1
+                    out.put(s, ("error", error))
+                    continue
                 self.stats["finished"] += 1
                 out.put(s, ("done", s.req.finish_reason))
             out.flush()
