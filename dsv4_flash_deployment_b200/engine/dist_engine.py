@@ -31,6 +31,7 @@ engine.py:602-632`` (``broadcast_one_to_all`` of a header + padded ids) and
 
 from __future__ import annotations
 
+import pickle
 import time
 from dataclasses import dataclass, field
 
@@ -54,6 +55,35 @@ class GlobalRequest:
     t_done: float | None = None
     logprobs: list = field(default_factory=list)   # per token when the request asked for them
     error: str | None = None      # why its rank's engine ended it
+
+
+@dataclass(frozen=True)
+class PickledGrammar:
+    """A request's grammar object on its way to the request's rank.  It is a pickle inside
+    the control message, so that an object which a rank cannot make again ends one
+    request there and not the rank."""
+
+    data: bytes
+
+    @staticmethod
+    def of(grammar) -> "PickledGrammar":
+        """ValueError for an object that does not come back from its pickle here."""
+        try:
+            p = PickledGrammar(pickle.dumps(grammar, protocol=pickle.HIGHEST_PROTOCOL))
+            p.make()
+        except Exception as e:  # noqa: BLE001  (whatever the object's own pickling raises)
+            raise ValueError(f"grammar: an object that can be pickled expected ({type(e).__name__}: {e})") from e
+        return p
+
+    def make(self):
+        return pickle.loads(self.data)
+
+
+def _travelling(rules: dict) -> dict:
+    """Checked rules as they go to the request's rank: the fields, not the masks."""
+    as_plain = {"logit_bias": lambda b: {int(t): float(v) for t, v in b.items()},
+                "allowed_token_ids": lambda ids: [int(t) for t in ids], "grammar": PickledGrammar.of}
+    return {k: as_plain.get(k, float)(v) for k, v in rules.items()}
 
 
 class _SchedView:
@@ -98,8 +128,15 @@ def _error(req) -> tuple:
 
 def _local_step(engine, msg: dict, rank: int, id_map: dict, pad_slot: int, replicated: bool = False) -> list[tuple]:
     """Applies a control message to this rank's engine and runs its part of the step."""
+    out = []
     for gid, r, prompt, mt, ignore_eos, stop_ids, temperature, extra in msg["adds"]:
         if r == rank or r == -1:
+            if isinstance(extra.get("grammar"), PickledGrammar):
+                try:
+                    extra = {**extra, "grammar": extra["grammar"].make()}
+                except Exception as e:  # noqa: BLE001  (the object's own code: only this request ends)
+                    out.append((gid, None, True, "cancelled", None, f"grammar: {type(e).__name__}: {e}"))
+                    continue
             req = engine.add_request(prompt, mt, ignore_eos=ignore_eos, stop_ids=stop_ids, temperature=temperature,
                                      **extra)
             id_map[req.req_id] = gid
@@ -116,7 +153,6 @@ def _local_step(engine, msg: dict, rank: int, id_map: dict, pad_slot: int, repli
         # no local forward ran: join the step's collectives with a 1-token step on the reserved slot
         engine.run_meta(StepMeta(engine.cfg, [SeqChunk(pad_slot, 0, [0], True)]))
         engine.stats["dummy_steps"] = engine.stats.get("dummy_steps", 0) + 1
-    out = []
     for req, tok in events:
         gid = id_map.get(req.req_id)
         lp = req.logprobs[len(req.output) - 1] if tok is not None and req.logprobs else None
@@ -164,8 +200,14 @@ class DistributedEngine:
             raise ValueError("empty prompt")
         # checked here, on rank 0, so that no rank is sent a request its engine refuses
         sp = self.local.sampling_params(temperature, top_k, top_p, logprobs, seed)
+        rules = {k: v for k, v in rules.items() if v is not None}
         if rules:
+            # what is checked is what travels: no iterator that is spent, no type of the caller's own
+            for name, plain in (("logit_bias", dict), ("allowed_token_ids", list)):
+                if name in rules:
+                    rules[name] = plain(rules[name])
             self.local.token_rules(**rules)
+            rules = _travelling(rules)
         if len(prompt) + max_new_tokens > self.local.sched.max_seq_len:
             raise ValueError(f"prompt {len(prompt)} + {max_new_tokens} new tokens exceeds max_seq_len "
                              f"{self.local.sched.max_seq_len}")
@@ -176,8 +218,7 @@ class DistributedEngine:
         g = GlobalRequest(self.next_id, r, list(prompt), max_new_tokens)
         extra = {} if not (sp.top_k or sp.top_p < 1.0 or sp.wants_logprobs or sp.seed is not None) else \
             {"top_k": sp.top_k, "top_p": sp.top_p, "logprobs": sp.logprobs, "seed": sp.seed}
-        extra = {**extra, **{k: v for k, v in rules.items() if v is not None}}   # the fields travel, not the masks
-        g._opts = (bool(ignore_eos), tuple(stop_ids), sp.temperature, extra)
+        g._opts = (bool(ignore_eos), tuple(stop_ids), sp.temperature, {**extra, **rules})
         self.next_id += 1
         self.load[r] += 1
         self.pending_adds.append(g)

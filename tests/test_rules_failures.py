@@ -109,3 +109,95 @@ def test_other_ranks_report_the_error():
     assert len(toks) == 1 and len(ends) == 1
     gid, tok, fin, reason, lp, error = ends[0]
     assert gid == 7 and tok is None and reason == "cancelled" and "KeyError" in error
+
+
+class NotToBeSent:
+    """Holds what cannot be pickled."""
+
+    def __init__(self):
+        self.f = lambda output: None
+
+    def mask(self, output):
+        return self.f(output)
+
+
+class NotToBeReceived:
+    """Pickles, but cannot be made again from its pickle."""
+
+    def __reduce__(self):
+        return (_refuse, ())
+
+    def mask(self, output):
+        return None
+
+
+class OnlyOnRankZero:
+    """A rank other than the first cannot make it from its pickle."""
+
+    def __init__(self, rank=0):
+        if rank != 0:
+            raise ImportError("not here")
+
+    def __reduce__(self):
+        return (_made_where, ())
+
+    def mask(self, output):
+        return None
+
+
+_RANK = [0]
+
+
+def _made_where():
+    return OnlyOnRankZero(_RANK[0])
+
+
+def _refuse():
+    raise ImportError("not to be had")
+
+
+def _rank_grammars(rank, world):
+    import torch.distributed as dist
+
+    from dsv4_flash_deployment_b200.engine.dist_engine import DistributedEngine, worker_loop
+    from dsv4_flash_deployment_b200.models.sampling import AllowedTokens
+
+    _RANK[0] = rank
+    eng = build_local_engine(EngineConfig(device="cpu", model="toy-v4", max_seqs=2, max_batched_tokens=32, chunk_size=16,
+                                          max_model_len=96), extra_slots=1)
+    if rank != 0:
+        return worker_loop(eng, dist.group.WORLD)
+    de = DistributedEngine(eng, dist.group.WORLD)
+    refused = 0
+    for g in (NotToBeSent(), NotToBeReceived()):
+        try:
+            de.add_request(P, 3, grammar=g)
+        except ValueError:
+            refused += 1
+    left = (len(de.pending_adds), sum(de.load), len(de.live))
+    ok = [de.add_request(P, 3, ignore_eos=True, grammar=AllowedTokens([20 + i], eng.cfg.vocab_size)) for i in range(2)]
+    lost = [de.add_request(P, 3, ignore_eos=True, grammar=OnlyOnRankZero()) for _ in range(2)]
+    odd = [de.add_request(P, 2, ignore_eos=True, allowed_token_ids=iter([30])),
+           de.add_request(P, 2, ignore_eos=True, logit_bias=zip(np.array([31]), np.array([1e30])),
+                          presence_penalty=np.float32(-1))]
+    while not all(r.finished for r in ok + lost + odd):
+        de.step()
+    again = de.generate([P], 2, ignore_eos=True)
+    de.shutdown()
+    return {"odd": [r.output for r in odd], "refused": refused, "left": left, "ok": [(r.rank, r.output, r.error) for r in ok], "loads": de.load,
+            "lost": {r.rank: (len(r.output), r.finish_reason, r.error) for r in lost}, "again": len(again[0])}
+
+
+def test_grammars_that_do_not_travel():
+    """Refused when the request is added; one that only another rank cannot make ends its
+    own request there and nothing else."""
+    from dsv4_flash_deployment_b200.utils.launch import spawn
+
+    res = spawn(_rank_grammars, 2, timeout_s=300)[0]
+    assert res["refused"] == 2 and res["left"] == (0, 0, 0)
+    assert sorted(res["ok"]) == [(0, [20] * 3, None), (1, [21] * 3, None)]
+    assert res["lost"][0] == (3, "length", None)
+    n, reason, error = res["lost"][1]
+    assert n == 0 and reason == "cancelled" and "not here" in error
+    assert res["odd"] == [[30, 30], [31, 31]]
+    assert res["again"] == 2 and res["loads"] == [0, 0]
