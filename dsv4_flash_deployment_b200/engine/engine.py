@@ -50,6 +50,8 @@ class Engine:
                  bucket: bool = True, max_graphs: int = 48, preempt: bool = False):
         self.model = model
         self.cfg = model.cfg
+        if hasattr(model, "alloc_rules") and model.tp is None:     # the vocab-parallel head takes no rules
+            model.alloc_rules()
         self.sched = Scheduler(max_seqs, max_batched_tokens, max_seq_len, chunk_size,
                                kv=getattr(model, "pager", None), preempt=preempt)
         self.use_graphs = use_graphs and model.dev.type == "cuda"

@@ -265,6 +265,50 @@ def token_bucket(n: int, cap: int) -> int:
 # --------------------------------------------------------------------------
 # model
 # --------------------------------------------------------------------------
+class RuleBuffers:
+    """Device buffers of the rules on logits: every slot's token history and the rules of a
+    step's sampled rows.  A sequence has one sampled row with rules a step, so masks and
+    biases are sized by slots (the last is the padding's)."""
+
+    def __init__(self, n_slots: int, max_tokens: int, max_sample: int, vocab: int, device):
+        seqs, i32, f32 = n_slots + 1, torch.int32, torch.float32
+        e = lambda *s, dt=i32: torch.empty(*s, dtype=dt, device=device)
+        self.history = TokenHistory.empty(seqs, vocab, device)
+        self.hist = e(max_tokens)
+        self.slot = e(max_sample)
+        self.penalties = tuple(e(max_sample, dt=f32) for _ in range(3))
+        self.mask_rows = e(max_sample)
+        self.masks = e(seqs * ((vocab + 31) // 32))
+        self.bias_off = e(max_sample + 1)
+        self.bias_ids = torch.zeros(seqs * MAX_BIAS, dtype=i32, device=device)
+        self.bias_vals = torch.zeros(seqs * MAX_BIAS, dtype=f32, device=device)
+        self.words = (vocab + 31) // 32
+
+    def tensors(self) -> list[torch.Tensor]:
+        return [self.history.seen, self.history.counts, self.hist, self.slot, *self.penalties, self.mask_rows, self.masks,
+                self.bias_off, self.bias_ids, self.bias_vals]
+
+    def upload(self, m: StepMeta, put) -> None:
+        for slot in m.resets:
+            self.history.reset(slot)
+        put(self.hist, m.hist)
+        put(self.slot, m.r_slot)
+        for dst, arr in zip(self.penalties, (m.r_rep, m.r_freq, m.r_pres)):
+            put(dst, arr)
+        put(self.mask_rows, m.mask_rows)
+        put(self.bias_off, m.bias_off)
+        if len(m.bias_ids):
+            put(self.bias_ids, m.bias_ids)
+            put(self.bias_vals, m.bias_vals)
+        if m.masks:
+            put(self.masks, np.concatenate(m.masks))
+
+    def rows(self, S: int) -> RowRules:
+        return (RowRules().penalties(self.slot[:S], *(t[:S] for t in self.penalties))
+                .biases(self.bias_off[:S + 1], self.bias_ids, self.bias_vals)
+                .masks(self.mask_rows[:S], self.masks.view(-1, self.words)))
+
+
 class DSV4Model:
     def __init__(self, cfg, layers: list[LayerW], embed: torch.Tensor, head: torch.Tensor, norm_w: torch.Tensor,
                  max_tokens: int, n_slots: int, max_seq_len: int, device, ep=None, max_sample: int | None = None,
@@ -532,7 +576,8 @@ class DSV4Model:
             put(self.m_seedkey, m.seedkey)
             put(self.m_hasseed, m.has_seed)
         if m.ruled:
-            self._upload_rules(m, put)
+            self.alloc_rules()
+            self.rules.upload(m, put)
         for r, g in m.groups.items():
             for dst, arr in zip(self.m_groups[r], g):
                 if len(arr):
@@ -540,40 +585,13 @@ class DSV4Model:
             put(self.m_clen[r], m.clen[r])
             put(self.m_ngroups[r], np.asarray([len(g[0])], np.int32))
 
-    history: TokenHistory | None = None     # tokens of every slot, for penalties
+    rules: RuleBuffers | None = None
 
-    def _upload_rules(self, m: StepMeta, put) -> None:
-        """Rules of the sampled rows; the buffers are made by the first step that has any."""
-        if self.history is None:
-            dev, S, V = self.dev, self.max_sample, self.vocab
-            i32, f32 = torch.int32, torch.float32
-            self.history = TokenHistory.empty(self.n_slots + 1, V, dev)
-            self.m_hist = torch.empty(self.max_tokens, dtype=i32, device=dev)
-            self.r_slot = torch.empty(S, dtype=i32, device=dev)
-            self.r_pen = tuple(torch.empty(S, dtype=f32, device=dev) for _ in range(3))
-            self.r_mask_rows = torch.empty(S, dtype=i32, device=dev)
-            self.r_masks = torch.empty(S * ((V + 31) // 32), dtype=i32, device=dev)
-            self.r_bias_off = torch.empty(S + 1, dtype=i32, device=dev)
-            self.r_bias_ids = torch.zeros(S * MAX_BIAS, dtype=i32, device=dev)
-            self.r_bias_vals = torch.zeros(S * MAX_BIAS, dtype=f32, device=dev)
-        for slot in m.resets:
-            self.history.reset(slot)
-        put(self.m_hist, m.hist)
-        put(self.r_slot, m.r_slot)
-        for dst, arr in zip(self.r_pen, (m.r_rep, m.r_freq, m.r_pres)):
-            put(dst, arr)
-        put(self.r_mask_rows, m.mask_rows)
-        put(self.r_bias_off, m.bias_off)
-        if len(m.bias_ids):
-            put(self.r_bias_ids, m.bias_ids)
-            put(self.r_bias_vals, m.bias_vals)
-        if m.masks:
-            put(self.r_masks, np.concatenate(m.masks))
-
-    def _row_rules(self, S: int) -> RowRules:
-        return (RowRules().penalties(self.r_slot[:S], *(t[:S] for t in self.r_pen))
-                .biases(self.r_bias_off[:S + 1], self.r_bias_ids, self.r_bias_vals)
-                .masks(self.r_mask_rows[:S], self.r_masks.view(self.max_sample, -1)))
+    def alloc_rules(self) -> None:
+        """Makes the buffers of the rules on logits.  The engine does this when it is built, so
+        that no step has to find memory for the first request that has rules."""
+        if self.rules is None:
+            self.rules = RuleBuffers(self.n_slots, self.max_tokens, self.max_sample, self.vocab, self.dev)
 
     last_upload_bytes = 0
     op_timer: dict | None = None
@@ -703,7 +721,7 @@ class DSV4Model:
                  norm=self.norm_w, u=self.u if self.head_q is None else None, tp=td)
         S = len(m.sample_rows)
         if m.ruled:     # this step's tokens join their slots' histories before any row reads them
-            self.history.add(self.m_ids[:T], self.m_slot[:T], self.m_hist[:T])
+            self.rules.history.add(self.m_ids[:T], self.m_slot[:T], self.rules.hist[:T])
         if S == 0:
             return self.next_ids[:0]
         with self._t("head"):
@@ -725,7 +743,7 @@ class DSV4Model:
                 self.lp_vals[:S, :n_top].copy_(vals)
                 self.lp_ids[:S, :n_top].copy_(ids)
             if m.ruled:
-                apply_logits_rules(self.logits[:S, :self.vocab], self._row_rules(S), self.history)
+                apply_logits_rules(self.logits[:S, :self.vocab], self.rules.rows(S), self.rules.history)
             if m.filtering:
                 top_k_top_p_mask_(self.logits[:S, :self.vocab], self.m_temp[:S], self.m_topk[:S], self.m_topp[:S])
             if m.sampling:
