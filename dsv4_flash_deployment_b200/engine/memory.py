@@ -12,6 +12,8 @@ from __future__ import annotations
 import torch
 
 from ..models.kv_format import ik4_bytes, kv4_bytes, kv8_bytes
+from ..models.sampling import MAX_BIAS
+from ..ops.layout import ceil_to
 
 
 def expert_block_bytes(cfg, ep_world: int = 1) -> int:
@@ -22,10 +24,25 @@ def expert_block_bytes(cfg, ep_world: int = 1) -> int:
     return int(e_local * per * (1 + 1 / 32))
 
 
+def rules_bytes(cfg, max_tokens: int, n_slots: int) -> int:
+    """The buffers of the rules on logits (models/model.py ``RuleBuffers``): a count and a
+    bit per slot and vocabulary entry, mask and biases per slot, the rows' parameters."""
+    words = (cfg.vocab_size + 31) // 32
+    per_slot = 4 * (cfg.vocab_size + 2 * words + 2 * MAX_BIAS)
+    return (n_slots + 1) * per_slot + 4 * (7 * max_tokens + 1)
+
+
+def head_int8_bytes(cfg, max_tokens: int) -> int:
+    """The int8 output head beside the bf16 one, and its quantized rows."""
+    d = ceil_to(cfg.dim, 16)
+    return ceil_to(cfg.vocab_size, 128) * (d + 4) + max_tokens * (d + 4)
+
+
 def non_expert_bytes(cfg, max_tokens: int, n_slots: int, max_seq: int, kv_block: int = 0,
-                     kv_pool_tokens: int = 0) -> int:
+                     kv_pool_tokens: int = 0, head_int8: bool = False, rules: bool = True) -> int:
     """``kv_block`` > 0: the compressed caches are paged pools of ``kv_pool_tokens``
-    tokens of context (0: ``n_slots * max_seq``) plus one scratch block per ratio."""
+    tokens of context (0: ``n_slots * max_seq``) plus one scratch block per ratio.
+    ``rules``: the engine takes rules on logits (not on the vocab-parallel head)."""
     d = cfg.dim
     per_layer = ((cfg.q_lora_rank + cfg.head_dim) * d + cfg.q_dim * cfg.q_lora_rank + 2 * cfg.o_inter * cfg.o_group_in
                  + d * cfg.o_inter + 3 * d * cfg.n_shared_experts * cfg.moe_inter_dim
@@ -54,19 +71,22 @@ def non_expert_bytes(cfg, max_tokens: int, n_slots: int, max_seq: int, kv_block:
     cap = t * k * 2 + cfg.n_routed_experts * 128
     step = (t * (cfg.hc_mult * d * 2 + 6 * d + 2 * 2 * cfg.q_dim + 6 * cfg.o_inter + 16 * cfg.head_dim)
             + cap * (d * 3 + cfg.moe_inter_dim * 2) + t * cfg.vocab_size * 4 + 64 * 2 ** 20)
-    return dense + emb + kv + step
+    extra = (head_int8_bytes(cfg, t) if head_int8 else 0) + (rules_bytes(cfg, t, n_slots) if rules else 0)
+    return dense + emb + kv + step + extra
 
 
 def plan_expert_storage(cfg, device, max_tokens: int, n_slots: int, max_seq: int, ep_world: int = 1,
-                        reserve_gb: float = 10.0) -> int:
+                        reserve_gb: float = 10.0, head_int8: bool = False, rules: bool = True) -> int:
     free, _ = torch.cuda.mem_get_info(device)
-    avail = free - non_expert_bytes(cfg, max_tokens, n_slots, max_seq) - int(reserve_gb * 2 ** 30)
+    avail = free - non_expert_bytes(cfg, max_tokens, n_slots, max_seq, head_int8=head_int8, rules=rules) - \
+        int(reserve_gb * 2 ** 30)
     n = int(avail // expert_block_bytes(cfg, ep_world))
     return max(1, min(cfg.n_layers, n))
 
 
 def kv_pool_tokens_for(cfg, total_bytes: int, utilization: float, max_tokens: int, n_slots: int, max_seq: int,
-                       kv_block: int, ep_world: int = 1, expert_layers: int | None = None) -> int:
+                       kv_block: int, ep_world: int = 1, expert_layers: int | None = None,
+                       head_int8: bool = False, rules: bool = True) -> int:
     """Tokens of context the paged compressed-cache pools can hold when the instance
     may use ``utilization`` of ``total_bytes`` of HBM (vLLM's
     ``--gpu-memory-utilization``, which the reference serves with at 0.85): the
@@ -79,8 +99,8 @@ def kv_pool_tokens_for(cfg, total_bytes: int, utilization: float, max_tokens: in
     layers = cfg.n_layers if expert_layers is None else expert_layers
     experts = layers * expert_block_bytes(cfg, ep_world)
     p0, p1 = max_seq, max_seq + (1 << 20)
-    b0 = non_expert_bytes(cfg, max_tokens, n_slots, max_seq, kv_block, p0)
-    b1 = non_expert_bytes(cfg, max_tokens, n_slots, max_seq, kv_block, p1)
+    b0 = non_expert_bytes(cfg, max_tokens, n_slots, max_seq, kv_block, p0, head_int8, rules)
+    b1 = non_expert_bytes(cfg, max_tokens, n_slots, max_seq, kv_block, p1, head_int8, rules)
     per_token = (b1 - b0) / (p1 - p0)
     spare = utilization * total_bytes - experts - b0
     pool = p0 + int(spare // per_token) if per_token > 0 else p0

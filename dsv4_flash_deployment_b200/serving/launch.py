@@ -37,7 +37,8 @@ def build_local_engine(ec: EngineConfig, ep=None, extra_slots: int = 0, tp=None)
 
         world = ep.world if ep is not None else (tp.world if tp is not None and tp.moe == "ep" else 1)
         storage = plan_expert_storage(cfg, torch.device(ec.device, torch.cuda.current_device()),
-                                      ec.max_batched_tokens, ec.max_seqs + extra_slots + 1, ec.max_model_len, world)
+                                      ec.max_batched_tokens, ec.max_seqs + extra_slots + 1, ec.max_model_len, world,
+                                      head_int8=ec.head_int8, rules=tp is None)
     pool = ec.kv_pool_tokens
     if ec.kv_block and not pool and ec.gpu_memory_utilization:
         # the paged pools take what the utilization leaves after the weights and buffers
@@ -48,7 +49,8 @@ def build_local_engine(ec: EngineConfig, ep=None, extra_slots: int = 0, tp=None)
         pool = kv_pool_tokens_for(cfg, torch.cuda.get_device_properties(dev).total_memory,
                                   ec.gpu_memory_utilization, ec.max_batched_tokens, ec.max_seqs + extra_slots + 1,
                                   ec.max_model_len, ec.kv_block, world,
-                                  expert_layers=None if weights is not None else storage)
+                                  expert_layers=None if weights is not None else storage,
+                                  head_int8=ec.head_int8, rules=tp is None)
     return Engine.build(cfg, device=ec.device, max_seqs=ec.max_seqs, max_batched_tokens=ec.max_batched_tokens,
                         max_seq_len=ec.max_model_len, weights=weights, seed=ec.seed,
                         expert_storage_layers=storage, ep=ep, use_graphs=ec.use_cuda_graphs,

@@ -50,3 +50,28 @@ def test_a_failed_allocation_leaves_nothing_half_made(monkeypatch):
     first = m.rules
     m.alloc_rules()
     assert m.rules is first and first.history.counts.shape == (3, 100)
+
+
+@pytest.mark.parametrize("slots,tokens", [(1, 8), (16, 64), (513, 1024)])
+def test_the_planner_counts_what_is_allocated(slots, tokens):
+    from dsv4_flash_deployment_b200.config import v4_flash_config
+    from dsv4_flash_deployment_b200.engine import memory
+
+    cfg = v4_flash_config() if slots < 100 else toy_v4_config()
+    b = RuleBuffers(slots, tokens, tokens, cfg.vocab_size, "cpu")
+    held = sum(t.numel() * t.element_size() for t in b.tensors())
+    assert memory.rules_bytes(cfg, tokens, slots) == held
+    plain = memory.non_expert_bytes(cfg, tokens, slots, 128, rules=False)
+    assert memory.non_expert_bytes(cfg, tokens, slots, 128) == plain + held
+    with_head = memory.non_expert_bytes(cfg, tokens, slots, 128, rules=False, head_int8=True)
+    assert with_head - plain >= cfg.vocab_size * (cfg.dim + 4) + tokens * (cfg.dim + 4)
+
+
+def test_the_pool_shrinks_by_what_the_rules_and_the_head_take():
+    from dsv4_flash_deployment_b200.config import v4_flash_config
+    from dsv4_flash_deployment_b200.engine import memory
+
+    cfg = v4_flash_config()
+    args = dict(max_tokens=1024, n_slots=513, max_seq=2048, kv_block=64, ep_world=8)
+    size = lambda **kw: memory.kv_pool_tokens_for(cfg, 178 * 2 ** 30, 0.85, **args, **kw)
+    assert size(rules=False) > size() > size(head_int8=True)
