@@ -23,7 +23,7 @@ from typing import Iterable
 import torch
 
 from ..models.model import DSV4Model, SeqChunk, StepMeta
-from ..models.sampling import SamplingParams, TokenRules, logprob_entries
+from ..models.sampling import NothingAllowed, SamplingParams, TokenRules, logprob_entries
 from ..ops.gemm import ErrorWord
 from .scheduler import Request, Scheduler
 
@@ -133,41 +133,51 @@ class Engine:
         return sp
 
     def step(self) -> list[tuple[Request, int | None]]:
-        chunks, masks, failed = self._masked(self.sched.schedule())
+        chunks, masks, ended = self._masked(self.sched.schedule())
         if not chunks:
-            return failed
+            return ended
         meta = StepMeta(self.cfg, [SeqChunk(c.req.slot, c.start_pos, c.tokens, c.sample,
                                             temperature=c.req.temperature, top_k=c.req.top_k, top_p=c.req.top_p,
                                             logprobs=c.req.want_logprobs, seed=c.req.seed, rules=c.req.rules,
                                             n_prompt=len(c.req.prompt), mask=m)
                                    for c, m in zip(chunks, masks)])
         ids = self.run_meta(meta)
+        if meta.ruled:
+            rows = [(c, m) for c, m in zip(chunks, masks) if c.sample]
+            for i, (c, m) in enumerate(rows):
+                if c.req.rules is not None and not c.req.rules.permits(ids[i], m):
+                    self.sched.fail(c.req, "the rules leave nothing: every allowed token's logit is -inf")
+                    ids[i] = None
         if meta.want_lp:
             it = iter(self.last_logprobs)
             for c in chunks:
                 if c.sample:
                     e = next(it)
-                    if e is not None:
+                    if e is not None and c.req.error is None:
                         c.req.logprobs.append(e)
-        return failed + self.sched.commit(chunks, ids)
+        return ended + self.sched.commit(chunks, ids)
 
     def _masked(self, chunks) -> tuple[list, list, list]:
-        """The chunks to run and the grammar mask of each (None: any token).  A request
-        whose grammar fails ends here, with its error and without a token; its event is
-        in the third list."""
-        run, masks, failed = [], [], []
+        """The chunks to run and the grammar mask of each (None: any token).  A request that
+        no token may follow ends here as it is, one whose grammar fails with its error;
+        its event (no token) is in the third list."""
+        run, masks, ended = [], [], []
         for c in chunks:
             mask = None
             if c.sample and c.req.rules is not None:
                 try:
                     mask = c.req.rules.words(c.req.output, self.cfg.vocab_size, self.eos_id)
+                except NothingAllowed:
+                    self.sched.stop(c.req)
+                    ended.append((c.req, None))
+                    continue
                 except Exception as e:  # noqa: BLE001  (a request's own grammar object: only that request ends)
                     self.sched.fail(c.req, f"grammar: {type(e).__name__}: {e}")
-                    failed.append((c.req, None))
+                    ended.append((c.req, None))
                     continue
             run.append(c)
             masks.append(mask)
-        return run, masks, failed
+        return run, masks, ended
 
     last_logprobs: list = []   # per sampled row of the last step that asked for log-probabilities
 

@@ -137,6 +137,10 @@ class Scheduler:
         req.error = error
         self._finish(req, "cancelled")
 
+    def stop(self, req: Request) -> None:
+        """Ends a request whose output is complete as it is."""
+        self._finish(req, "stop")
+
     def schedule(self) -> list[ScheduledChunk]:
         # drop cancelled requests
         for r in [r for r in self.running if r.cancelled]:
@@ -216,8 +220,9 @@ class Scheduler:
         self.n_preempted += 1
         self.waiting.appendleft(r)
 
-    def commit(self, chunks: list[ScheduledChunk], next_ids: list[int]) -> list[tuple[Request, int | None]]:
-        """Applies a step's results; returns (request, new token or None) per chunk."""
+    def commit(self, chunks: list[ScheduledChunk], next_ids: list[int | None]) -> list[tuple[Request, int | None]]:
+        """Applies a step's results (None: the row's request has failed); returns (request,
+        new token or None) per chunk."""
         events = []
         it = iter(next_ids)
         now = time.perf_counter()

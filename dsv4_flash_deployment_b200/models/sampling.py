@@ -18,6 +18,7 @@ reaches ``p`` (at least one token).
 
 from __future__ import annotations
 
+import functools
 import math
 from dataclasses import dataclass
 
@@ -25,7 +26,12 @@ import numpy as np
 import torch
 
 LOGPROB_TOP_N = 20   # most alternatives a request may ask for (the OpenAI API's top_logprobs limit)
+BIAS_LIMIT = 3.4028235677973366e38   # values from here on round to infinity in fp32
 MAX_BIAS = 300       # most biased tokens of a request (the limit vLLM's and OpenAI's servers document)
+
+
+class NothingAllowed(ValueError):
+    """A grammar that no token may follow, not even the end of sequence."""
 
 
 class AllowedTokens:
@@ -71,6 +77,11 @@ class TokenRules:
     def penalizes(self) -> bool:
         return self.repetition != 1.0 or self.frequency != 0.0 or self.presence != 0.0
 
+    @functools.cached_property
+    def banned(self) -> np.ndarray:
+        """Tokens whose bias is -inf (in the fp32 that is added)."""
+        return np.array([t for t, b in self.bias if b <= -BIAS_LIMIT], np.int64)
+
     @staticmethod
     def make(vocab: int, repetition_penalty: float | None = None, frequency_penalty: float | None = None,
              presence_penalty: float | None = None, logit_bias=None, allowed_token_ids=None,
@@ -94,7 +105,7 @@ class TokenRules:
             t, b = int(k), float(v)
             if not 0 <= t < vocab:
                 raise ValueError(f"logit_bias: token {t} is outside the vocabulary of {vocab}")
-            if math.isnan(b) or b > 3.4e38:
+            if math.isnan(b) or b >= BIAS_LIMIT:
                 raise ValueError("logit_bias values must be finite or -inf")
             if t in bias:
                 raise ValueError(f"logit_bias: token {t} is given twice")
@@ -108,11 +119,30 @@ class TokenRules:
         if grammar is not None and not callable(getattr(grammar, "mask", None)):
             raise ValueError("grammar: an object with mask(output) expected")
         r = TokenRules(rep, freq, pres, tuple(sorted(bias.items())), grammar)
+        if len(r.banned) >= vocab:
+            raise ValueError("logit_bias: every token is banned")
+        if isinstance(grammar, AllowedTokens):     # the same mask at every position
+            try:
+                r.words([], vocab, None)
+            except NothingAllowed:
+                raise ValueError("allowed_token_ids: logit_bias has banned every one of them") from None
         return r if r.penalizes or r.bias or r.grammar is not None else None
 
+    def _keep(self, w: np.ndarray, vocab: int) -> np.ndarray:
+        """Mask words without the banned tokens and without bits past the vocabulary."""
+        past = int(w.view(np.uint32)[-1]) >> vocab % 32 if vocab % 32 else 0
+        if not (past or len(self.banned)):
+            return w
+        bits = w.view(np.uint32).copy()
+        if past:
+            bits[-1] &= np.uint32((1 << vocab % 32) - 1)
+        np.bitwise_and.at(bits, self.banned >> 5, ~(np.uint32(1) << (self.banned & 31).astype(np.uint32)))
+        return bits.view(np.int32)
+
     def words(self, output, vocab: int, eos_id: int | None) -> np.ndarray | None:
-        """Mask words for the token that follows ``output`` (None: any).  A grammar that
-        allows nothing leaves the end of sequence."""
+        """Mask words for the token that follows ``output`` (None: any), without banned
+        tokens.  Where that leaves nothing the end of sequence remains; NothingAllowed
+        where there is none or it is banned too."""
         if self.grammar is None:
             return None
         w = self.grammar.mask(output)
@@ -122,14 +152,19 @@ class TokenRules:
         n = (vocab + 31) // 32
         if w.ndim != 1 or w.size < n or w.dtype not in (np.int32, np.uint32):
             raise ValueError(f"grammar mask: {n} int32 words expected")
-        w = w[:n].view(np.int32)
-        if vocab % 32:
-            last = w.view(np.uint32)[-1] & np.uint32((1 << vocab % 32) - 1)
-            if not w[:-1].any() and not last:
-                w = np.zeros(n, np.int32)
-        if not w.any() and eos_id is not None and 0 <= eos_id < vocab:
-            return token_words([eos_id], vocab)
-        return w
+        w = self._keep(w[:n].view(np.int32), vocab)
+        if w.any():
+            return w
+        if eos_id is None or not 0 <= eos_id < vocab or eos_id in self.banned:
+            raise NothingAllowed("the grammar allows no token")
+        return token_words([eos_id], vocab)
+
+    def permits(self, token: int, mask: np.ndarray | None) -> bool:
+        """Whether a sampled token is one that the mask and the biases leave: not so where
+        every logit of the row is -inf."""
+        if mask is not None and not int(mask[token >> 5]) >> (token & 31) & 1:
+            return False
+        return token not in self.banned
 
 
 @dataclass(frozen=True)

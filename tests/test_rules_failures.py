@@ -8,6 +8,7 @@ import pytest
 
 from dsv4_flash_deployment_b200.engine.config import EngineConfig
 from dsv4_flash_deployment_b200.engine.dist_engine import _local_step
+from dsv4_flash_deployment_b200.models.sampling import AllowedTokens, NothingAllowed, TokenRules, token_words
 from dsv4_flash_deployment_b200.serving.engine_loop import EngineLoop, GenParams
 from dsv4_flash_deployment_b200.serving.launch import build_local_engine
 
@@ -201,3 +202,73 @@ def test_grammars_that_do_not_travel():
     assert n == 0 and reason == "cancelled" and "not here" in error
     assert res["odd"] == [[30, 30], [31, 31]]
     assert res["again"] == 2 and res["loads"] == [0, 0]
+
+
+# ------------------------------------------------------- rows where nothing is left
+NINF = float("-inf")
+
+
+def test_an_allowed_list_that_is_wholly_banned_is_refused():
+    eng = _engine()
+    v = eng.cfg.vocab_size
+    for kw in (dict(allowed_token_ids=[65], logit_bias={65: NINF}), dict(allowed_token_ids=[65], logit_bias={65: -1e39}),
+               dict(allowed_token_ids=[5, 6], logit_bias={6: NINF, 5: NINF, 7: 1.0})):
+        with pytest.raises(ValueError, match="banned"):
+            eng.add_request(P, 3, **kw)
+        with pytest.raises(ValueError):
+            TokenRules.make(v, **kw)
+    with pytest.raises(ValueError, match="words"):       # made for a smaller vocabulary
+        TokenRules.make(v, grammar=AllowedTokens([2], 40), logit_bias={v - 1: NINF})
+    with pytest.raises(ValueError, match="banned"):
+        TokenRules.make(40, logit_bias={t: NINF for t in range(40)})
+    # one of two is left, and a large finite value does not ban
+    out = _run(eng, [eng.add_request(P, 3, ignore_eos=True, allowed_token_ids=[5, 6], logit_bias={5: NINF}),
+                     eng.add_request(P, 3, ignore_eos=True, allowed_token_ids=[9], logit_bias={9: -1e30})])
+    assert out == [[6] * 3, [9] * 3]
+
+
+def test_banned_tokens_leave_the_mask():
+    g = lambda w: type("G", (), {"mask": lambda s, o: np.array(w, np.uint32)})()
+    r = TokenRules.make(70, logit_bias={3: NINF, 33: NINF, 34: 1.0, 1: -4e38}, grammar=g([0b1010, 0b110, 0]))
+    assert r.words([], 70, 2).tolist() == [0, 0b100, 0]
+    r = TokenRules.make(70, logit_bias={3: NINF, 33: NINF, 34: NINF, 1: NINF}, grammar=g([0b1010, 0b110, 1 << 6]))
+    assert r.words([], 70, 2).tolist() == [4, 0, 0]           # the end of sequence; bit 70 is past the end
+    for eos in (None, 3, -1, 70):
+        with pytest.raises(NothingAllowed):
+            r.words([], 70, eos)
+
+
+class _Ends:
+    """Token 40 once, then nothing."""
+
+    def __init__(self, vocab):
+        self.v = vocab
+
+    def mask(self, output):
+        return token_words([40], self.v) if not output else np.zeros((self.v + 31) // 32, np.int32)
+
+
+@pytest.mark.parametrize("how", ["banned", "none"])
+def test_the_request_ends_where_nothing_may_follow(how):
+    """With no end of sequence to give, the output is complete without one."""
+    eng = _engine()
+    bias = {eng.eos_id: NINF} if how == "banned" else None
+    if how == "none":
+        eng.eos_id = None
+    other = eng.add_request(P, 6, ignore_eos=True)
+    r = eng.add_request(P, 6, ignore_eos=True, grammar=_Ends(eng.cfg.vocab_size), logit_bias=bias)
+    _run(eng, [r, other])
+    assert r.output == [40] and r.finish_reason == "stop" and r.error is None and len(other.output) == 6
+    assert _idle(eng) and eng.generate([P], 3, grammar=_Ends(eng.cfg.vocab_size), logit_bias=bias) == [[40]]
+
+
+@pytest.mark.parametrize("extra", [{}, dict(temperature=1.0, seed=3), dict(temperature=1.0, top_k=5), dict(logprobs=2)])
+def test_penalties_that_leave_nothing_end_the_request(extra):
+    """The one allowed token's logit goes to -inf in the penalty: nothing is sampled in its place."""
+    eng = _engine()
+    kw = dict(allowed_token_ids=[P[3]], frequency_penalty=3e38, ignore_eos=True, **extra)
+    r, other = eng.add_request(P, 6, **kw), eng.add_request(P, 6, ignore_eos=True)
+    _run(eng, [r, other])
+    # counted once it is at -3e38, counted twice at -inf
+    assert r.output == [P[3]] * 2 and "nothing" in r.error and r.finish_reason == "cancelled"
+    assert len(r.logprobs) == (2 if "logprobs" in extra else 0) and len(other.output) == 6 and _idle(eng)
