@@ -132,7 +132,7 @@ def _params(st: ServerState, body: dict, n_prompt: int, chat: bool = False) -> t
         seed = None if body.get("seed") is None else int(body["seed"])
         sp = SamplingParams(temp, max(top_k, 0), top_p, lp, seed)     # top_k -1 (vLLM's "off") counts as 0
         rules = _rules_fields(body)
-    except (TypeError, ValueError) as e:
+    except (TypeError, ValueError, OverflowError) as e:
         raise web.HTTPBadRequest(text=json.dumps({"error": str(e)}), content_type="application/json") from None
     return (GenParams(mt, bool(body.get("ignore_eos", False)), stop_ids, temp, sp.top_k, sp.top_p, sp.logprobs,
                       sp.seed, rules),

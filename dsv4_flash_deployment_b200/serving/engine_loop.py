@@ -151,7 +151,7 @@ class EngineLoop:
                     kw.update(p.rules)
                     req = eng.add_request(prompt, p.max_tokens, ignore_eos=p.ignore_eos, stop_ids=p.stop_ids,
                                           temperature=p.temperature, **kw)
-                except (ValueError, TypeError) as e:
+                except (ValueError, TypeError, OverflowError) as e:
                     s.put(("error", str(e)))
                     continue
                 s.req = req
