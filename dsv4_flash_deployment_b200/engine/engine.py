@@ -110,7 +110,8 @@ class Engine:
 
     def token_rules(self, **rules) -> TokenRules | None:
         """Checked rules on a request's logits (ValueError when this engine cannot apply
-        them: they need the whole vocabulary's logits on one GPU)."""
+        them: the vocab-parallel head does not; each rule acts on one column, so its
+        shards could, from their first column on, but that is not built)."""
         unknown = set(rules) - {"repetition_penalty", "frequency_penalty", "presence_penalty", "logit_bias",
                                 "allowed_token_ids", "grammar"}
         if unknown:

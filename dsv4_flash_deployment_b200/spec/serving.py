@@ -23,6 +23,7 @@ import itertools
 from collections import deque
 
 from ..engine.scheduler import Request
+from ..models.sampling import TokenRules
 
 
 class _Queue:
@@ -79,7 +80,7 @@ class SpecServingEngine:
     def add_request(self, prompt: list[int], max_new_tokens: int, ignore_eos: bool = False,
                     stop_ids=(), temperature: float = 0.0, top_k: int = 0, top_p: float = 1.0,
                     logprobs: int | None = None, seed: int | None = None, **rules) -> Request:
-        if rules:
+        if TokenRules.make(self.cfg.vocab_size, **rules) is not None:
             raise ValueError("speculative decoding (DSpark) does not take penalties, logit_bias or grammars")
         if temperature > 0:
             raise ValueError("speculative decoding (DSpark) decodes greedily; temperature > 0 is not supported")

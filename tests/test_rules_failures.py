@@ -272,3 +272,18 @@ def test_penalties_that_leave_nothing_end_the_request(extra):
     # counted once it is at -3e38, counted twice at -inf
     assert r.output == [P[3]] * 2 and "nothing" in r.error and r.finish_reason == "cancelled"
     assert len(r.logprobs) == (2 if "logprobs" in extra else 0) and len(other.output) == 6 and _idle(eng)
+
+
+def test_speculative_decoding_takes_rules_that_do_nothing():
+    from types import SimpleNamespace
+
+    from dsv4_flash_deployment_b200.spec.serving import SpecServingEngine
+
+    cfg = _engine().cfg
+    eng = SpecServingEngine(SimpleNamespace(cfg=cfg, max_seqs=1, blk=4, open_rows=lambda: None), 96)
+    eng.add_request(P, 4, repetition_penalty=1.0, frequency_penalty=None, logit_bias={})
+    for kw in (dict(repetition_penalty=1.1), dict(allowed_token_ids=[1]), dict(logit_bias={1: 0.5})):
+        with pytest.raises(ValueError, match="speculative"):
+            eng.add_request(P, 4, **kw)
+    with pytest.raises(TypeError):
+        eng.add_request(P, 4, penalty=2.0)
