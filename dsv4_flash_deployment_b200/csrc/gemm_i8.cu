@@ -327,7 +327,7 @@ done:
 // A warp takes R weight rows and all T tokens; lane l reads the 16-byte pieces l,
 // l + 32, .. of a row, the tokens' pieces from L1/L2 beside it, four dp4a a piece
 // and token, and the lanes' sums meet in one integer warp reduction.  Four rows a warp
-// where the rows fill the SMs several times, else one, for more loads in flight.
+// or one (launch_rows).
 // One token, 129280 x 4096: 80 us (6.6 TB/s; the tensor-core tiles 83); 1280 x 5120:
 // 3.5 us (tiles 5.0, of which most is getting started: barriers, TMEM, the first TMA).
 template <int T, int R, typename TO>
@@ -635,7 +635,12 @@ cudaError_t launch_rows(const int8_t* x, size_t ldx, const int8_t* w, size_t ldw
     const unsigned grid = (unsigned)((p.N + 8 * rows - 1) / (8 * rows));
     return launch_pdl(kernel, grid, 256, 0, st, x, ldx, w, ldw, p);
   };
-  if (p.N >= 4 * 32 * sms) return go(gemm_i8_rows_kernel<T, 4, TO>, 4);
+  // Four rows a warp share the tokens' pieces, one row has eight pieces of its own in flight
+  // where K reaches 4096.  us with one and with four rows, one token: 5000 x 2048 4.2 and 5.1,
+  // 9000 x 2048 6.6 and 5.9, 40000 x 2048 19.2 and 16.6; 19000 x 4096 14.5 and 18.7, 40000 x
+  // 4096 27.7 and 30.6, 90000 x 4096 58.1 and 57.0; two tokens: 9000 x 2048 6.9 and 6.7, 40000 x
+  // 4096 34.3 and 34.2, 65536 x 4096 55.1 and 47.7 (19000 rows of K below 4096 up to 13 % off).
+  if (p.N >= (p.K < 4096 ? 56 : 440) * sms) return go(gemm_i8_rows_kernel<T, 4, TO>, 4);
   return go(gemm_i8_rows_kernel<T, 1, TO>, 1);
 }
 
