@@ -84,3 +84,48 @@ def test_int8_head_against_the_bf16_head(graphs):
         # the int8 head's token is one the bf16 head gives about as much to
         assert float(la[ta] - la[tb]) <= float(tol[ta] + tol[tb])
     assert len(prompts) == 3
+
+
+def test_int8_head_under_speculative_decoding():
+    """Drafted tokens are verified by the int8 head: the stream is that head's greedy one
+    (up to near-ties between the 1-token and the 5-token path, as with the bf16 head)."""
+    from dsv4_flash_deployment_b200.engine.builder import build_model
+    from dsv4_flash_deployment_b200.io.checkpoint_spec import make_random_weights
+    from dsv4_flash_deployment_b200.spec.dspark import SpecEngine
+
+    from test_dspark_gpu import _greedy, spec_cfg
+
+    cfg = spec_cfg()
+    w = make_random_weights(cfg, seed=6)
+    prompts = [torch.randint(0, 1000, (n,), generator=torch.Generator().manual_seed(n)).tolist() for n in (19, 26)]
+    kw = dict(max_tokens=64, n_slots=4, max_seq_len=128, weights=w, head_int8=True)
+    want = _greedy(build_model(cfg, "cuda", **kw), cfg, prompts[0], 20)
+    eng = SpecEngine(build_model(cfg, "cuda", **kw), w, max_seqs=4)
+    got = eng.generate(prompts, 20)
+    _done()
+    assert sum(int(a == b) for a, b in zip(got[0], want)) >= 18 and len(got[1]) == 20 and eng.stats.rounds > 0
+
+
+@pytest.mark.parametrize("graphs", [True, False])
+def test_histories_start_over_after_a_preemption(graphs):
+    """A preempted request's context is prefilled again, its own output with it: a token of
+    either is counted once, so none comes twice under a penalty that forbids it."""
+    from dsv4_flash_deployment_b200.engine.engine import Engine
+
+    cfg = small_v4()
+    eng = Engine.build(cfg, "cuda", max_seqs=3, max_batched_tokens=64, max_seq_len=128, seed=3, chunk_size=24,
+                       use_graphs=graphs, kv_block=4, kv_pool_tokens=160, kv_preempt=True)
+    n = 40
+    reqs = [eng.add_request(p, n, ignore_eos=True, presence_penalty=1e6, logit_bias={5: float("-inf")})
+            for p in _prompts(cfg)]
+    counted = []
+    while not all(r.finished for r in reqs):
+        eng.step()
+        live = [r for r in reqs if r.slot >= 0 and r.output and r.prompt_done]
+        counted += [(r, eng.model.rules.history.counts[r.slot].sum().item(), len(r.output)) for r in live]
+    eng.check_errors()
+    assert sum(r.preemptions for r in reqs) > 0
+    for r in reqs:
+        assert len(r.output) == n and len(set(r.output)) == n and 5 not in r.output
+    # after a step the last token is not in the history yet; every other one is, once
+    assert counted and all(c == k - 1 for _, c, k in counted)
