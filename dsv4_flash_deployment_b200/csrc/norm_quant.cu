@@ -714,7 +714,7 @@ static cudaError_t launch_norm(const NormQuantParams& p, bool vec, int sms, cuda
   if (!vec || p.D > 2 * 8 * kNormThreads) {
     // 8 to 32 columns a thread, as many as it takes for the rows to be resident together (1024
     // threads an SM), and 256 threads, four blocks an SM, rather than two of up to 384 (fp32
-    // 777 x 5003 9.9 us with 16, 8.4 so; 9598 x 6177 166 and 144; 4096 x 8200 59 and 48; bf16
+    // 777 x 5003 9.9 us with 16, 8.2 so; 9598 x 6177 166 and 144; 4096 x 8200 59 and 44; bf16
     // 2000 x 12001 54.6 and 49.0; 777 x 1001 5.2 and 4.2).
     auto warps = [](int n) { return std::max(32, (n + 31) / 32 * 32); };
     const int fit = 1024 / std::min(32, (p.T + sms - 1) / sms) / 32 * 32;
@@ -767,8 +767,8 @@ static cudaError_t launch_norm(const NormQuantParams& p, bool vec, int sms, cuda
     }
   }
   // 16-bit rows: two blocks of 512 threads an SM (64 registers; 16384 x 4096 bf16 to MXFP8
-  // 108 us, with one block an SM 139), and one group a thread up to 6144 columns (512 x 5120
-  // to MXFP8 7.8 us, with two groups a thread 8.8; to int8 5.9 and 6.1)
+  // 111 us, with one block an SM 139), and one group a thread up to 6144 columns (512 x 5120
+  // to MXFP8 8.0 us, with two groups a thread 8.8; to int8 5.9 and 6.1)
   const int nt1 = (groups + 31) / 32 * 32;
   if constexpr (sizeof(TX) == 2) {
     if (groups <= kNormThreads) DSV4_NQ(false, 1, nt1, 1, kNormThreads, 2);
